@@ -15,6 +15,7 @@
 #include <unordered_map>
 
 #include "attention.h"
+#include "bindings_kv8.h"
 #include "peer_ring.h"
 #include "gemm.h"
 #include "gemm_fp8.h"
@@ -855,4 +856,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("EPI_SILU") = static_cast<int>(atlas::kEpiSilu);
   m.attr("EPI_F32") = static_cast<int>(atlas::kEpiF32);
   m.attr("EPI_PEER") = static_cast<int>(atlas::kEpiPeer);
+  register_kv8(m);
 }

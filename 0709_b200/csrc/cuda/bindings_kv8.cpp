@@ -1,0 +1,235 @@
+// Python bindings of the 8-bit KV cache kernels.  Outputs and split records are allocated here, on
+// the current stream (no workspace outlives a call, so calls on several streams and captured graphs
+// share nothing), and every launch status becomes an exception.
+
+#include "bindings_kv8.h"
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <algorithm>
+
+#include "attention.h"
+#include "kv8.h"
+
+namespace {
+
+constexpr double kLog2e = 1.4426950408889634;
+
+// data [.., pages, 2, Hkv, ps, 128] e4m3 with scale of the leading dimensions; returns log2(page size).
+int check_cache(const torch::Tensor& data, const torch::Tensor& scale, int64_t dim) {
+  TORCH_CHECK(data.is_cuda() && data.dim() == dim && data.is_contiguous() &&
+                  data.scalar_type() == torch::kFloat8_e4m3fn,
+              "the 8-bit cache must be a contiguous float8_e4m3fn CUDA tensor of ", dim, " dimensions");
+  TORCH_CHECK(data.size(-1) == 128 && data.size(-4) == 2, "the 8-bit cache kernels need [.., 2, Hkv, page, 128]");
+  const int64_t ps = data.size(-2);
+  TORCH_CHECK(ps == 8 || ps == 16 || ps == 32 || ps == 64, "the 8-bit cache kernels need pages of 8, 16, 32 or 64 slots");
+  TORCH_CHECK(scale.scalar_type() == torch::kFloat32 && scale.is_contiguous() && scale.device() == data.device() &&
+                  scale.sizes() == data.sizes().slice(0, dim - 2),
+              "the 8-bit cache needs one float32 scale per page, side and head on its device");
+  TORCH_CHECK(data.numel() / 128 < (int64_t{1} << 31) && data.size(-5) > 0 && data.size(-3) > 0, "8-bit cache size");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, "the 8-bit cache must be 16-byte aligned");
+  return ps == 8 ? 3 : ps == 16 ? 4 : ps == 32 ? 5 : 6;
+}
+
+void check_int(const torch::Tensor& t, const torch::Tensor& like, const char* name, int64_t n = -1) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == torch::kInt32 && t.is_contiguous(), name,
+              " must be a contiguous int32 tensor on the cache's device");
+  TORCH_CHECK(n < 0 || t.numel() == n, name, " must hold ", n, " values, not ", t.numel());
+}
+
+void check_err(const torch::Tensor& err, const torch::Tensor& like) {
+  TORCH_CHECK(err.device() == like.device() && err.scalar_type() == torch::kInt32 && err.numel() >= 1,
+              "the op table belongs to ", err.device(), ", the cache to ", like.device());
+}
+
+void check_launch(cudaError_t e, const char* what) {
+  TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
+}
+
+uint8_t* bytes(const torch::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
+
+torch::Tensor kv8_append(torch::Tensor qkv, torch::Tensor table, torch::Tensor pos, torch::Tensor slots,
+                         torch::Tensor data, torch::Tensor scale, int64_t Hq, int64_t out_bf16, torch::Tensor err) {
+  const int shift = check_cache(data, scale, 5);
+  check_err(err, data);
+  const int64_t Hkv = data.size(2), M = qkv.size(0);
+  const auto t = qkv.scalar_type();
+  TORCH_CHECK(t == torch::kHalf || t == torch::kBFloat16 || t == torch::kFloat32, "qkv must be fp16, bf16 or fp32");
+  TORCH_CHECK(qkv.device() == data.device() && qkv.dim() == 2 && Hq >= 1 && qkv.size(1) == (Hq + 2 * Hkv) * 128,
+              "qkv must be [M, (Hq + 2 Hkv) * 128] on the cache's device");
+  if (qkv.stride(1) != 1 || (M > 1 && qkv.stride(0) % 4 != 0) || reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 != 0)
+    qkv = qkv.clone(at::MemoryFormat::Contiguous);
+  TORCH_CHECK(table.device() == data.device() && table.scalar_type() == torch::kFloat32 && table.is_contiguous() &&
+                  table.dim() == 2 && table.size(1) == 128 && table.size(0) < (int64_t{1} << 31) &&
+                  reinterpret_cast<uintptr_t>(table.data_ptr()) % 16 == 0,
+              "the rotary table must be contiguous fp32 [positions, 128] on the cache's device");
+  check_int(pos, data, "positions", M);
+  check_int(slots, data, "slots", M);
+  TORCH_CHECK(M < (int64_t{1} << 31) && (Hq + 3) / 4 + Hkv <= 65535, "kv8 append size");
+  const bool bf16 = t == torch::kFloat32 ? out_bf16 != 0 : t == torch::kBFloat16;
+  const c10::cuda::CUDAGuard guard(data.device());
+  auto q = torch::empty({M, Hq, 128}, qkv.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf));
+  atlas::Kv8AppendParams p{};
+  p.qkv = qkv.data_ptr();
+  p.table = table.data_ptr<float>();
+  p.pos = pos.data_ptr<int>();
+  p.slots = slots.data_ptr<int>();
+  p.data = bytes(data);
+  p.scale = scale.data_ptr<float>();
+  p.q_out = q.data_ptr();
+  p.err = err.data_ptr<int>();
+  p.ld = qkv.stride(0);
+  p.M = static_cast<int>(M);
+  p.Hq = static_cast<int>(Hq);
+  p.Hkv = static_cast<int>(Hkv);
+  p.page_shift = shift;
+  p.num_pages = static_cast<int>(data.size(0));
+  p.max_pos = static_cast<int>(table.size(0));
+  p.in_type = t == torch::kFloat32 ? atlas::kKv8F32 : t == torch::kBFloat16 ? atlas::kKv8Bf16 : atlas::kKv8F16;
+  p.out_bf16 = bf16 ? 1 : 0;
+  check_launch(atlas::launch_kv8_append(p, at::cuda::getCurrentCUDAStream()), "kv8_append");
+  return q;
+}
+
+void kv8_copy_pages(torch::Tensor data, torch::Tensor scale, torch::Tensor plan, c10::optional<torch::Tensor> count,
+                    torch::Tensor err) {
+  const int shift = check_cache(data, scale, 6);
+  check_err(err, data);
+  check_int(plan, data, "the copy plan");
+  TORCH_CHECK(plan.dim() == 2 && plan.size(1) == 3, "the copy plan must be [n, 3]");
+  if (count.has_value()) {
+    check_int(*count, data, "the copy count");
+    TORCH_CHECK(count->numel() >= 1, "the copy count must hold one value");
+  }
+  TORCH_CHECK(data.size(0) <= 65535 && 2 * data.size(3) <= 65535, "kv8 copy size");
+  const c10::cuda::CUDAGuard guard(data.device());
+  check_launch(atlas::launch_kv8_copy_pages(bytes(data), scale.data_ptr<float>(), plan.data_ptr<int>(),
+                                            count.has_value() ? count->data_ptr<int>() : nullptr,
+                                            static_cast<int>(plan.size(0)), static_cast<int>(data.size(0)),
+                                            static_cast<int>(data.size(1)), static_cast<int>(data.size(3)), shift,
+                                            err.data_ptr<int>(), at::cuda::getCurrentCUDAStream()),
+               "kv8_copy_pages");
+}
+
+void kv8_move_slots(torch::Tensor data, torch::Tensor scale, torch::Tensor src, torch::Tensor dst, torch::Tensor err) {
+  const int shift = check_cache(data, scale, 6);
+  check_err(err, data);
+  check_int(src, data, "source slots");
+  check_int(dst, data, "destination slots", src.numel());
+  TORCH_CHECK(src.numel() <= atlas::kKv8MaxMoves, "at most ", atlas::kKv8MaxMoves, " slot moves per call, not ",
+              src.numel());
+  TORCH_CHECK(2 * data.size(3) <= 65535, "kv8 move size");
+  const c10::cuda::CUDAGuard guard(data.device());
+  check_launch(atlas::launch_kv8_move_slots(bytes(data), scale.data_ptr<float>(), src.data_ptr<int>(),
+                                            dst.data_ptr<int>(), static_cast<int>(src.numel()),
+                                            static_cast<int>(data.size(0)), static_cast<int>(data.size(1)),
+                                            static_cast<int>(data.size(3)), shift, err.data_ptr<int>(),
+                                            at::cuda::getCurrentCUDAStream()),
+               "kv8_move_slots");
+}
+
+// One layer (data of 5 dimensions) -> [n, 2, Hkv, ps, 128]; a whole cache (6) -> [L, n, 2, Hkv, ps, 128].
+torch::Tensor kv8_read_pages(torch::Tensor data, torch::Tensor scale, torch::Tensor pages, bool bf16,
+                             torch::Tensor err) {
+  const bool layers = data.dim() == 6;
+  const int shift = check_cache(data, scale, layers ? 6 : 5);
+  check_err(err, data);
+  check_int(pages, data, "pages");
+  const int64_t L = layers ? data.size(0) : 1, n = pages.numel(), Hkv = data.size(-3), ps = data.size(-2);
+  TORCH_CHECK(L <= 65535 && 2 * Hkv <= 65535, "kv8 read size");
+  const c10::cuda::CUDAGuard guard(data.device());
+  const auto opt = data.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf);
+  auto out = layers ? torch::empty({L, n, 2, Hkv, ps, 128}, opt) : torch::empty({n, 2, Hkv, ps, 128}, opt);
+  check_launch(atlas::launch_kv8_read_pages(bytes(data), scale.data_ptr<float>(), pages.data_ptr<int>(),
+                                            out.data_ptr(), static_cast<int>(n), static_cast<int>(L),
+                                            static_cast<int>(data.size(-5)), static_cast<int>(Hkv), shift, bf16,
+                                            err.data_ptr<int>(), at::cuda::getCurrentCUDAStream()),
+               "kv8_read_pages");
+  return out;
+}
+
+// Splits of the shared keys: enough CTAs to fill the device, at least 128 keys each, 64 at most.
+int64_t pick_splits8(int64_t tiles, int64_t keys, int sms) {
+  return std::max<int64_t>(1, std::min<int64_t>({64, sms / std::max<int64_t>(tiles, 1), (keys + 127) / 128}));
+}
+
+std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data, torch::Tensor scale, c10::optional<torch::Tensor> dparams,
+                         int64_t shared_len, int64_t n_shared_pages, int64_t mask_base, torch::Tensor prefix_pages,
+                         torch::Tensor row_full, torch::Tensor row_len, torch::Tensor row_mask, torch::Tensor tail_pages,
+                         double softmax_scale, int64_t max_keys, torch::Tensor err) {
+  const int shift = check_cache(data, scale, 5);
+  check_err(err, data);
+  TORCH_CHECK(q.device() == data.device() && q.dim() == 3 && q.size(2) == 128 &&
+                  (q.scalar_type() == torch::kHalf || q.scalar_type() == torch::kBFloat16),
+              "q must be fp16 or bf16 [M, Hq, 128] on the cache's device");
+  if (!q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
+    q = q.clone(at::MemoryFormat::Contiguous);
+  const int64_t M = q.size(0), Hq = q.size(1), Hkv = data.size(2);
+  TORCH_CHECK(Hq >= 1 && Hq % Hkv == 0, "Hq must be a multiple of Hkv");
+  TORCH_CHECK(M * Hq < (int64_t{1} << 31), "attention8 size");
+  check_int(prefix_pages, data, "prefix_pages");
+  check_int(row_full, data, "row_full", M);
+  check_int(row_len, data, "row_len", M);
+  TORCH_CHECK(row_mask.device() == data.device() && row_mask.scalar_type() == torch::kInt64 &&
+                  row_mask.is_contiguous() && row_mask.dim() == 2 && row_mask.size(0) == M,
+              "row_mask must be contiguous int64 [M, words] on the cache's device");
+  check_int(tail_pages, data, "tail_pages");
+  TORCH_CHECK(tail_pages.dim() == 2 && tail_pages.size(0) == M, "tail_pages must be [M, T]");
+  TORCH_CHECK(shared_len >= 0 && n_shared_pages >= 0 && std::max(shared_len, n_shared_pages << shift) < (1 << 30),
+              "shared_len and n_shared_pages must be positions below 2^30");
+  if (dparams.has_value()) {
+    check_int(*dparams, data, "the descriptor's device scalars");
+    TORCH_CHECK(dparams->numel() >= 3, "the descriptor's device scalars are shared_len, n_shared_pages, mask_base");
+  }
+  const c10::cuda::CUDAGuard guard(data.device());
+  auto out = torch::empty({M, Hq * 128}, q.options());
+  if (M == 0) return {out, 0};
+  atlas::Attn8Params p{};
+  p.q = q.data_ptr();
+  p.data = bytes(data);
+  p.scale = scale.data_ptr<float>();
+  p.out = out.data_ptr();
+  p.dparams = dparams.has_value() ? dparams->data_ptr<int>() : nullptr;
+  p.shared_len = static_cast<int>(shared_len);
+  p.n_shared_pages = static_cast<int>(n_shared_pages);
+  p.mask_base = static_cast<int>(mask_base);
+  p.prefix_pages = prefix_pages.data_ptr<int>();
+  p.row_full = row_full.data_ptr<int>();
+  p.row_len = row_len.data_ptr<int>();
+  p.row_mask = row_mask.data_ptr<int64_t>();
+  p.tail_pages = tail_pages.data_ptr<int>();
+  p.err = err.data_ptr<int>();
+  p.M = static_cast<int>(M);
+  p.Hq = static_cast<int>(Hq);
+  p.Hkv = static_cast<int>(Hkv);
+  p.page_shift = shift;
+  p.num_pages = static_cast<int>(data.size(0));
+  p.n_prefix = static_cast<int>(prefix_pages.numel());
+  p.mask_words = static_cast<int>(row_mask.size(1));
+  p.tail_stride = static_cast<int>(tail_pages.size(1));
+  p.bf16 = q.scalar_type() == torch::kBFloat16;
+  p.scale_log2 = static_cast<float>(softmax_scale * kLog2e);
+  // A captured call is sized for the longest context its graph may see (max_keys), an eager one for its own.
+  const int64_t keys = std::max<int64_t>({shared_len, n_shared_pages << shift, max_keys});
+  p.splits = static_cast<int>(
+      keys > 0 || dparams.has_value() ? pick_splits8(Hkv, keys, at::cuda::getCurrentDeviceProperties()->multiProcessorCount) : 0);
+  torch::Tensor parts;
+  if (p.splits > 0) {
+    parts = torch::empty({p.splits * M * Hq * 130}, q.options().dtype(torch::kFloat32));
+    p.part_o = parts.data_ptr<float>();
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<int64_t>(p.splits) * M * Hq * 128);
+  }
+  check_launch(atlas::launch_attention8(CUtensorMap{}, p, at::cuda::getCurrentCUDAStream()), "attention8");
+  return {out, p.splits > 0 ? 2 : 1};
+}
+
+}  // namespace
+
+void register_kv8(pybind11::module& m) {
+  m.def("kv8_append", &kv8_append, "rotary embedding and rounding of k and v into the 8-bit cache; returns rotated q");
+  m.def("kv8_copy_pages", &kv8_copy_pages, "copies of partial pages in every layer of the 8-bit cache");
+  m.def("kv8_move_slots", &kv8_move_slots, "slot moves in every layer of the 8-bit cache (sources read first)");
+  m.def("kv8_read_pages", &kv8_read_pages, "pages of the 8-bit cache as fp16 or bf16 values");
+  m.def("attention8", &attention8, "paged attention over one layer of the 8-bit cache");
+}

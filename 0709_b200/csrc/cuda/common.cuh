@@ -23,6 +23,7 @@ enum ErrorCode : int {
   kErrBadIndex = 2,      // an index (page, slot, token) was out of range
   kErrConfig = 3,        // unsupported shape reached a kernel
   kErrPeerTimeout = 4,   // a peer GPU's flag did not arrive within the time limit
+  kErrNonFinite = 5,     // a value that the 8-bit cache cannot hold (NaN, infinite, too large)
 };
 
 __device__ __forceinline__ void set_error(int* flag, int code) {

@@ -1,0 +1,418 @@
+// 8-bit paged KV cache: append (rotary + rounding), page copies, slot moves, read back.
+//
+// An element stands for code * scale with e4m3 codes and one power-of-two scale per page, side
+// (k, v) and head.  Powers of two make every step exact but the one rounding to e4m3: x / scale is
+// exact, re-rounding a page after its scale grew changes only codes that fall below e4m3's smallest
+// normal number, and a page whose scale did not change is never touched.  The scale a row needs is
+// 2^e with the smallest e in [-40, 56] for which max |x| <= 448 * 2^e.
+//
+// Writing slots of a page (append and moves alike): the page's scale becomes the largest its new
+// rows need, or keeps its old value if that is larger, and the codes of its other slots are rounded
+// again when it grew.  Writing slot 0 starts the page anew: the scale is that of its new rows alone
+// and its other slots read zero, so a recycled page carries nothing of its last use.
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "kv8.h"
+#include "launch.h"
+
+namespace atlas {
+
+namespace {
+constexpr int kHd = 128;
+constexpr int kMaxPage = 64;
+constexpr int kExpMin = -40, kExpMax = 56;
+constexpr float kF16Max = 65504.f;
+}  // namespace
+
+__device__ __forceinline__ float kv8_pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// Exponent of the scale for max |x| given as its bits (448 = 1.75 * 2^8).
+__device__ __forceinline__ int kv8_exponent(uint32_t amax_bits) {
+  const int ex = static_cast<int>(amax_bits >> 23) - 127;
+  return max(kExpMin, ex - ((amax_bits & 0x7fffffu) <= 0x600000u ? 8 : 7));
+}
+__device__ __forceinline__ bool kv8_storable(uint32_t amax_bits) {
+  return amax_bits < 0x7f800000u && kv8_exponent(amax_bits) <= kExpMax;
+}
+
+__device__ __forceinline__ uint32_t kv8_encode4(const float* x, float inv) {
+  const uint32_t lo =
+      __nv_cvt_float2_to_fp8x2(make_float2(x[0] * inv, x[1] * inv), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi =
+      __nv_cvt_float2_to_fp8x2(make_float2(x[2] * inv, x[3] * inv), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+__device__ __forceinline__ void kv8_decode4(uint32_t w, float* x) {
+  const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffff), __NV_E4M3);
+  const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3);
+  const float2 fa = __half22float2(__half2(a)), fb = __half22float2(__half2(b));
+  x[0] = fa.x;
+  x[1] = fa.y;
+  x[2] = fb.x;
+  x[3] = fb.y;
+}
+// The codes of w rounded again for a scale larger by 1 / ratio (ratio <= 1, a power of two).
+__device__ __forceinline__ uint32_t kv8_rescale4(uint32_t w, float ratio) {
+  float x[4];
+  kv8_decode4(w, x);
+  return kv8_encode4(x, ratio);
+}
+
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* x) {
+  const uint2 r = *reinterpret_cast<const uint2*>(p);
+  const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = to_f32(e[i]);
+}
+template <>
+__device__ __forceinline__ void load4<float>(const float* p, float* x) {
+  *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(p);
+}
+
+// a * b - c * d with the error of the second product put back (two roundings in all): near a
+// rounding border of e4m3 a plain fp32 difference would more often fall on the wrong side.
+__device__ __forceinline__ float diff_of_products(float a, float b, float c, float d) {
+  const float cd = c * d;
+  const float err = fmaf(-c, d, cd);
+  return fmaf(a, b, -cd) + err;
+}
+
+// Lane l's four rotated values, dimensions 4 l .. 4 l + 3, of the head at x (rotate-half pairing:
+// dimension i < 64 pairs with i + 64).
+template <typename T>
+__device__ __forceinline__ void rotate4(const T* x, const float* cs, int lane, float* y) {
+  const int i = (lane & 15) * 4;
+  float a[4], b[4], c[4], s[4];
+  load4<T>(x + i, a);
+  load4<T>(x + 64 + i, b);
+  load4<float>(cs + i, c);
+  load4<float>(cs + 64 + i, s);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    y[e] = lane < 16 ? diff_of_products(a[e], c[e], b[e], s[e]) : diff_of_products(b[e], c[e], -a[e], s[e]);
+}
+
+__device__ __forceinline__ uint32_t abs_bits_max4(const float* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+  return m;
+}
+
+template <typename O>
+__device__ __forceinline__ void store4(O* p, const float* x) {
+  O v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = from_f32<O>(x[e]);
+  *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
+}
+
+// grid (M, ceil(Hq / 4) + Hkv), 128 threads.  Query blocks: one warp per head.  KV blocks: the first
+// row of the batch that writes a page (the others leave at once) handles all of the page's rows for
+// one kv head, so each page and head has one writer and no order of blocks matters; a row whose
+// predecessor writes the same page -- 15 of 16 in a prompt -- leaves without a scan of the slots.
+template <typename T, typename O>
+__global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
+  __shared__ int owner[kMaxPage];  // row that writes slot o, -1: none
+  __shared__ uint32_t amax_s[2];
+  __shared__ int follower;
+  pdl_wait();
+  pdl_trigger();
+  const int m = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int qblocks = (p.Hq + 3) / 4;
+  const T* qkv = static_cast<const T*>(p.qkv);
+  if (static_cast<int>(blockIdx.y) < qblocks) {
+    const int head = blockIdx.y * 4 + warp;
+    if (head >= p.Hq) return;
+    const int pos = p.pos[m];
+    float y[4] = {0.f, 0.f, 0.f, 0.f};
+    if (pos >= 0 && pos < p.max_pos)
+      rotate4<T>(qkv + m * p.ld + head * kHd, p.table + static_cast<int64_t>(pos) * kHd, lane, y);
+    else if (lane == 0)
+      set_error(p.err, kErrBadIndex);
+    store4<O>(static_cast<O*>(p.q_out) + (static_cast<int64_t>(m) * p.Hq + head) * kHd + lane * 4, y);
+    return;
+  }
+  const int h = blockIdx.y - qblocks;
+  const int slot = p.slots[m];
+  const int page = slot >> p.page_shift;
+  const int ps = 1 << p.page_shift;
+  if (slot < 0 || page >= p.num_pages) {
+    if (tid == 0) set_error(p.err, kErrBadIndex);
+    return;
+  }
+  if (m > 0) {
+    const int before = p.slots[m - 1];
+    if (before >= 0 && (before >> p.page_shift) == page) return;
+  }
+  if (tid < kMaxPage) owner[tid] = -1;
+  if (tid < 2) amax_s[tid] = 0;
+  if (tid == 0) follower = 0;
+  __syncthreads();
+  for (int j = tid; j < p.M; j += 128) {
+    const int s = p.slots[j];
+    if (s >= 0 && (s >> p.page_shift) == page) {
+      if (j < m) follower = 1;
+      atomicMax(&owner[s & (ps - 1)], j);
+    }
+  }
+  float* scale = p.scale + (static_cast<int64_t>(page) * 2) * p.Hkv + h;
+  const float old_k = scale[0], old_v = scale[p.Hkv];
+  __syncthreads();
+  if (follower) return;
+  // Largest magnitudes of the new rows; a row that cannot be stored is reported and left out.
+  for (int o = warp; o < ps; o += 4) {
+    const int r = owner[o];
+    if (r < 0) continue;  // warp-uniform
+    const int pos = p.pos[r];
+    bool ok = pos >= 0 && pos < p.max_pos;
+    int code = kErrBadIndex;
+    if (ok) {
+      float k[4], v[4];
+      const T* row = qkv + r * p.ld;
+      rotate4<T>(row + (p.Hq + h) * kHd, p.table + static_cast<int64_t>(pos) * kHd, lane, k);
+      load4<T>(row + (p.Hq + p.Hkv + h) * kHd + lane * 4, v);
+      const uint32_t ak = __reduce_max_sync(0xffffffffu, abs_bits_max4(k));
+      const uint32_t av = __reduce_max_sync(0xffffffffu, abs_bits_max4(v));
+      ok = kv8_storable(ak) && kv8_storable(av);
+      code = kErrNonFinite;
+      if (ok && lane == 0) {
+        atomicMax(&amax_s[0], ak);
+        atomicMax(&amax_s[1], av);
+      }
+    }
+    if (!ok && lane == 0) {
+      set_error(p.err, code);
+      owner[o] = -1;
+    }
+  }
+  __syncthreads();
+  const bool anew = owner[0] >= 0;
+  bool any = false;
+  for (int o = 0; o < ps; ++o) any |= owner[o] >= 0;
+  if (!any) return;
+  const float need_k = kv8_pow2(kv8_exponent(amax_s[0])), need_v = kv8_pow2(kv8_exponent(amax_s[1]));
+  const float new_k = anew ? need_k : fmaxf(old_k, need_k);
+  const float new_v = anew ? need_v : fmaxf(old_v, need_v);
+  const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
+  uint32_t* kd = reinterpret_cast<uint32_t*>(p.data) +
+                 ((static_cast<int64_t>(page) * 2) * p.Hkv + h) * ps * (kHd / 4) + lane;
+  uint32_t* vd = kd + static_cast<int64_t>(p.Hkv) * ps * (kHd / 4);
+  for (int o = warp; o < ps; o += 4) {
+    const int r = owner[o];
+    uint32_t* ko = kd + o * (kHd / 4);
+    uint32_t* vo = vd + o * (kHd / 4);
+    if (r >= 0) {
+      float k[4], v[4];
+      const T* row = qkv + r * p.ld;
+      rotate4<T>(row + (p.Hq + h) * kHd, p.table + static_cast<int64_t>(p.pos[r]) * kHd, lane, k);
+      load4<T>(row + (p.Hq + p.Hkv + h) * kHd + lane * 4, v);
+      *ko = kv8_encode4(k, inv_k);
+      *vo = kv8_encode4(v, inv_v);
+    } else if (anew) {
+      *ko = 0;
+      *vo = 0;
+    } else {
+      if (new_k > old_k && old_k > 0.f) *ko = kv8_rescale4(*ko, old_k * inv_k);
+      if (new_v > old_v && old_v > 0.f) *vo = kv8_rescale4(*vo, old_v * inv_v);
+    }
+  }
+  if (tid == 0) {
+    scale[0] = new_k;
+    scale[p.Hkv] = new_v;
+  }
+}
+
+// grid (min(n, 64), layers, 2 * Hkv).  Copies of one call are independent: a destination that is
+// also a source, or twice a destination, is reported and skipped.  The slots behind the copied ones
+// are zeroed; a copy of no token leaves an empty page (scale 0), which is how a page is freed.
+__global__ void __launch_bounds__(128)
+    kv8_copy_pages_kernel(uint4* __restrict__ data, float* __restrict__ scale, const int* __restrict__ plan,
+                          const int* __restrict__ count, int max_n, int num_pages, int Hkv, int page_shift, int* err) {
+  pdl_wait();
+  pdl_trigger();
+  const int n = count != nullptr ? min(*count, max_n) : max_n;
+  const int ps = 1 << page_shift;
+  const int64_t layer = blockIdx.y;
+  const int kvh = blockIdx.z;
+  const int vec = ps * (kHd / 16);
+  for (int ci = blockIdx.x; ci < n; ci += gridDim.x) {
+    const int src = plan[ci * 3 + 0], dst = plan[ci * 3 + 1], ntok = plan[ci * 3 + 2];
+    bool bad = src < 0 || src >= num_pages || dst < 0 || dst >= num_pages || ntok < 0 || ntok > ps || src == dst;
+    for (int j = threadIdx.x; j < n; j += blockDim.x)
+      if (j != ci && (plan[j * 3] == dst || plan[j * 3 + 1] == dst)) bad = true;
+    if (__syncthreads_or(bad)) {
+      if (threadIdx.x == 0) set_error(err, kErrBadIndex);
+      continue;
+    }
+    const int64_t s = (layer * num_pages + src) * 2 * Hkv + kvh, d = (layer * num_pages + dst) * 2 * Hkv + kvh;
+    const int keep = ntok * (kHd / 16);
+    for (int i = threadIdx.x; i < vec; i += blockDim.x)
+      data[d * vec + i] = i < keep ? data[s * vec + i] : make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) scale[d] = ntok > 0 ? scale[s] : 0.f;
+  }
+}
+
+// grid (layers, 2 * Hkv), 256 threads; shared memory: n codes rows, scales, slots, page tables.
+// Every source is read before any slot is written; then one warp per destination page.
+__global__ void __launch_bounds__(256)
+    kv8_move_slots_kernel(uint8_t* __restrict__ data, float* __restrict__ scale, const int* __restrict__ src,
+                          const int* __restrict__ dst, int n, int num_pages, int Hkv, int page_shift, int* err) {
+  extern __shared__ uint4 buf[];
+  uint32_t* rows = reinterpret_cast<uint32_t*>(buf);  // [n][32]
+  float* from = reinterpret_cast<float*>(rows + n * 32);
+  int* to = reinterpret_cast<int*>(from + n);
+  __shared__ int owners[8][kMaxPage];
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ps = 1 << page_shift;
+  const int64_t layer = blockIdx.x;
+  const int64_t head = layer * num_pages * 2 * Hkv + blockIdx.y;  // + page * 2 Hkv: page-head index
+  for (int j = warp; j < n; j += 8) {
+    const int s = src[j], d = dst[j];
+    const bool ok = s >= 0 && (s >> page_shift) < num_pages && d >= 0 && (d >> page_shift) < num_pages;
+    if (ok) {
+      const int64_t ph = head + static_cast<int64_t>(s >> page_shift) * 2 * Hkv;
+      rows[j * 32 + lane] = *reinterpret_cast<const uint32_t*>(data + (ph * ps + (s & (ps - 1))) * kHd + lane * 4);
+      if (lane == 0) from[j] = scale[ph];
+    } else if (lane == 0) {
+      set_error(err, kErrBadIndex);
+    }
+    if (lane == 0) to[j] = ok ? d : -1;
+  }
+  __syncthreads();
+  int* owner = owners[warp];
+  for (int j = warp; j < n; j += 8) {
+    const int d = to[j];
+    if (d < 0) continue;
+    const int page = d >> page_shift;
+    bool seen = false;  // an earlier move of this page handles it
+    for (int i = lane; i < j; i += 32) seen |= to[i] >= 0 && (to[i] >> page_shift) == page;
+    if (__any_sync(0xffffffffu, seen)) continue;
+    owner[lane] = -1;
+    owner[lane + 32] = -1;
+    __syncwarp();
+    for (int i = j + lane; i < n; i += 32)
+      if (to[i] >= 0 && (to[i] >> page_shift) == page) atomicMax(&owner[to[i] & (ps - 1)], i);  // the later move wins
+    __syncwarp();
+    float need = 0.f;
+    for (int o = lane; o < ps; o += 32)
+      if (owner[o] >= 0) need = fmaxf(need, from[owner[o]]);
+    need = warp_max(need);
+    const bool anew = owner[0] >= 0;
+    const int64_t ph = head + static_cast<int64_t>(page) * 2 * Hkv;
+    const float old = scale[ph];
+    const float now = anew ? need : fmaxf(old, need);
+    const float inv = now > 0.f ? 1.f / now : 0.f;
+    uint32_t* out = reinterpret_cast<uint32_t*>(data + ph * ps * kHd) + lane;
+    for (int o = 0; o < ps; ++o) {
+      const int i = owner[o];
+      if (i >= 0)
+        out[o * 32] = from[i] == now ? rows[i * 32 + lane] : kv8_rescale4(rows[i * 32 + lane], from[i] * inv);
+      else if (anew)
+        out[o * 32] = 0;
+      else if (now > old && old > 0.f)
+        out[o * 32] = kv8_rescale4(out[o * 32], old * inv);
+    }
+    __syncwarp();  // every lane has read `old` and the owners
+    if (lane == 0) scale[ph] = now;
+  }
+}
+
+template <typename O>
+__device__ __forceinline__ O kv8_value(float x);
+template <>
+__device__ __forceinline__ __half kv8_value<__half>(float x) {
+  return __float2half_rn(fminf(fmaxf(x, -kF16Max), kF16Max));
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 kv8_value<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// grid (n, layers, 2 * Hkv): one page and head, 16 codes per thread and step.  fp16 values are held
+// to its largest finite number (rounding up to e4m3 can pass it).
+template <typename O>
+__global__ void __launch_bounds__(128)
+    kv8_read_pages_kernel(const uint4* __restrict__ data, const float* __restrict__ scale,
+                          const int* __restrict__ pages, O* __restrict__ out, int num_pages, int Hkv, int page_shift,
+                          int* err) {
+  pdl_wait();
+  pdl_trigger();
+  const int64_t layer = blockIdx.y;
+  const int kvh = blockIdx.z;
+  const int vec = (1 << page_shift) * (kHd / 16);
+  const int page = pages[blockIdx.x];
+  const bool ok = page >= 0 && page < num_pages;
+  if (!ok && threadIdx.x == 0) set_error(err, kErrBadIndex);
+  const int64_t s = (layer * num_pages + (ok ? page : 0)) * 2 * Hkv + kvh;
+  const float sc = ok ? scale[s] : 0.f;
+  uint4* o = reinterpret_cast<uint4*>(out) +
+             ((layer * gridDim.x + blockIdx.x) * 2 * Hkv + kvh) * static_cast<int64_t>(vec) * 2;
+  for (int i = threadIdx.x; i < vec; i += blockDim.x) {
+    const uint4 w = ok ? data[s * vec + i] : make_uint4(0, 0, 0, 0);
+    const uint32_t c[4] = {w.x, w.y, w.z, w.w};
+    O v[16];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float x[4];
+      kv8_decode4(c[e], x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[e * 4 + k] = kv8_value<O>(x[k] * sc);
+      }
+    }
+    o[2 * i] = reinterpret_cast<const uint4*>(v)[0];
+    o[2 * i + 1] = reinterpret_cast<const uint4*>(v)[1];
+  }
+}
+
+cudaError_t launch_kv8_append(const Kv8AppendParams& p, cudaStream_t st) {
+  if (p.M == 0) return cudaSuccess;
+  const dim3 grid(p.M, (p.Hq + 3) / 4 + p.Hkv);
+  if (p.in_type == kKv8Bf16) return launch_k(kv8_append_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, st, p);
+  if (p.in_type == kKv8F16) return launch_k(kv8_append_kernel<__half, __half>, grid, dim3(128), 0, st, p);
+  if (p.out_bf16) return launch_k(kv8_append_kernel<float, __nv_bfloat16>, grid, dim3(128), 0, st, p);
+  return launch_k(kv8_append_kernel<float, __half>, grid, dim3(128), 0, st, p);
+}
+
+cudaError_t launch_kv8_copy_pages(uint8_t* data, float* scale, const int* plan, const int* count, int n, int layers,
+                                  int num_pages, int Hkv, int page_shift, int* err, cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  const dim3 grid(count != nullptr ? 1 : (n < 64 ? n : 64), layers, 2 * Hkv);
+  return launch_k(kv8_copy_pages_kernel, grid, dim3(128), 0, st, reinterpret_cast<uint4*>(data), scale, plan, count, n,
+                  num_pages, Hkv, page_shift, err);
+}
+
+cudaError_t launch_kv8_move_slots(uint8_t* data, float* scale, const int* src, const int* dst, int n, int layers,
+                                  int num_pages, int Hkv, int page_shift, int* err, cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  const size_t smem = static_cast<size_t>(n) * (kHd + 8);
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kv8_move_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kKv8MaxMoves * (kHd + 8));
+    if (e != cudaSuccess) return e;
+  }
+  return launch_k(kv8_move_slots_kernel, dim3(layers, 2 * Hkv), dim3(256), smem, st, data, scale, src, dst, n,
+                  num_pages, Hkv, page_shift, err);
+}
+
+cudaError_t launch_kv8_read_pages(const uint8_t* data, const float* scale, const int* pages, void* out, int n,
+                                  int layers, int num_pages, int Hkv, int page_shift, bool bf16, int* err,
+                                  cudaStream_t st) {
+  if (n == 0) return cudaSuccess;
+  const dim3 grid(n, layers, 2 * Hkv);
+  const uint4* d = reinterpret_cast<const uint4*>(data);
+  if (bf16)
+    return launch_k(kv8_read_pages_kernel<__nv_bfloat16>, grid, dim3(128), 0, st, d, scale, pages,
+                    static_cast<__nv_bfloat16*>(out), num_pages, Hkv, page_shift, err);
+  return launch_k(kv8_read_pages_kernel<__half>, grid, dim3(128), 0, st, d, scale, pages, static_cast<__half*>(out),
+                  num_pages, Hkv, page_shift, err);
+}
+
+}  // namespace atlas

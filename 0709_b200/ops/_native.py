@@ -77,6 +77,9 @@ CUDA_SOURCES = [
     "tp.cu",
     "peer_ring.cu",
     "gemm_fp8.cu",
+    "bindings_kv8.cpp",
+    "kv8.cu",
+    "attention8.cu",
 ]
 
 

@@ -301,6 +301,94 @@ class CudaOps:
         self.ext.kv_move_slots(kv, src.to(self.device, torch.int32), dst.to(self.device, torch.int32), self.err)
         counters.launches(1)
 
+    # --------------------------------------------------- 8-bit KV cache
+    # Semantics in ``ops.kv8``.  Outputs and split records are allocated by each call on the current stream:
+    # no workspace is shared between streams, calls or captured graphs.
+    @staticmethod
+    def _int32(t: torch.Tensor) -> torch.Tensor:
+        return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
+    def rope_qkv_append8(self, qkv, table, positions, slots, kv_layer, num_heads, num_kv_heads, out_dtype=None):
+        """Rotate q/k, round k and v into the layer's pages at ``slots`` (one launch); returns q [M, Hq, 128] in
+        ``qkv``'s dtype, or in ``out_dtype`` (fp16 by default) when ``qkv`` is fp32."""
+        if num_kv_heads != kv_layer.data.shape[-3]:
+            raise ValueError(f"{num_kv_heads} kv heads for a cache of {kv_layer.data.shape[-3]}")
+        if out_dtype is None:
+            out_dtype = torch.float16 if qkv.dtype == torch.float32 else qkv.dtype
+        if out_dtype not in (torch.float16, torch.bfloat16) or qkv.dtype not in (out_dtype, torch.float32):
+            raise TypeError(f"rope_qkv_append8 writes q in fp16 or bf16, not {out_dtype} from {qkv.dtype}")
+        q = self.ext.kv8_append(qkv, table, self._int32(positions), self._int32(slots), kv_layer.data, kv_layer.scale,
+                                num_heads, out_dtype == torch.bfloat16, self.err)
+        counters.launches(1)
+        return q
+
+    def attention8(self, q: torch.Tensor, kv_layer, desc: AttnDesc, scale: float | None = None) -> torch.Tensor:
+        """Attention of q [M, Hq, 128] over one layer of the 8-bit cache per the descriptor; [M, Hq * 128] in q's
+        dtype.  A row that sees no key answers zero."""
+        scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+        out, launches = self.ext.attention8(
+            q, kv_layer.data, kv_layer.scale, getattr(desc, "_dparams", None), desc.shared_len, desc.n_shared_pages,
+            desc.mask_base, desc.prefix_pages, desc.row_full, desc.row_len, desc.row_mask, desc.tail_pages, scale,
+            getattr(desc, "_max_keys", 0), self.err,
+        )
+        counters.launches(launches)
+        return out
+
+    def attention8_causal(self, q, kv_layer, desc: AttnDesc, causal_start: int, scale: float | None = None):
+        """Attention of a prefill chunk at positions ``causal_start ..`` whose own keys are in the 8-bit cache.
+
+        Compute-bound, so it runs on the tensor-core kernel of the 16-bit cache: the sequence's pages are read once
+        into a 16-bit scratch of the chunk's own (exact values, freed with the call), a cost of a few microseconds
+        per thousand keys.
+        """
+        m, hq, hd = q.shape
+        scale = 1.0 / math.sqrt(hd) if scale is None else scale
+        out = torch.empty((m, hq * hd), dtype=q.dtype, device=q.device)
+        if m == 0:
+            return out
+        ps = kv_layer.data.shape[-2]
+        total = int(causal_start) + m
+        n = (total + ps - 1) // ps
+        if causal_start < 0 or n > desc.prefix_pages.numel():
+            raise ValueError(f"{total} positions need {n} pages of {ps} slots; the descriptor lists "
+                             f"{desc.prefix_pages.numel()}")
+        pages = self._int32(desc.prefix_pages[:n])
+        limit = torch.arange(int(causal_start) + 1, total + 1, dtype=torch.int32, device=q.device)
+        listed = torch.arange(n, dtype=torch.int32, device=q.device)
+        dparams = torch.tensor([total, n, 0], dtype=torch.int32).to(q.device)
+        # The attention kernel reads its index inputs before it waits for the kernel before it, which is the read.
+        scratch = self.ext.kv8_read_pages(kv_layer.data, kv_layer.scale, pages, q.dtype == torch.bfloat16, self.err)
+        self.ext.attention(
+            q.contiguous(), scratch[None], 0, out, dparams, listed, limit, limit, desc.row_mask, desc.tail_pages,
+            self.part_o, self.part_ml, self.err, 1, True, False, True, float(scale), False,
+        )
+        counters.launches(2)
+        return out
+
+    def kv8_copy_pages(self, cache, copies: torch.Tensor) -> None:
+        """Fork: rows (src page, dst page, ntok) of ``copies``; every layer, scales included."""
+        self.ext.kv8_copy_pages(cache.data, cache.scale, self._int32(copies.to(self.device)), None, self.err)
+        counters.launches(1)
+
+    def kv8_copy_pages_counted(self, cache, plan: torch.Tensor, count: torch.Tensor) -> None:
+        """``kv8_copy_pages`` of ``count[0]`` rows of ``plan`` [max, 3] (both read on the device)."""
+        self.ext.kv8_copy_pages(cache.data, cache.scale, plan, count, self.err)
+        counters.launches(1)
+
+    def kv8_move_slots(self, cache, src: torch.Tensor, dst: torch.Tensor) -> None:
+        """Compaction: slot contents move in every layer, sources read before any write; at most 1024 moves."""
+        self.ext.kv8_move_slots(cache.data, cache.scale, self._int32(src.to(self.device)),
+                                self._int32(dst.to(self.device)), self.err)
+        counters.launches(1)
+
+    def kv8_read_pages(self, cache, pages: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+        """The values of ``pages`` in fp16 or bf16: [n, 2, Hkv, page, 128] of a layer, [L, n, ...] of a cache."""
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"kv8_read_pages gives fp16 or bf16, not {dtype}")
+        out = self.ext.kv8_read_pages(cache.data, cache.scale, self._int32(pages), dtype == torch.bfloat16, self.err)
+        counters.launches(1)
+        return out
+
     # ----------------------------------------------------------- vocab
     def topk_logprobs(self, logits: torch.Tensor, k: int, keys: torch.Tensor | None = None, temperature: float = 1.0):
         b = logits.shape[0]

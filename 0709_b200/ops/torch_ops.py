@@ -17,6 +17,7 @@ import math
 import torch
 
 from ..models.llama import GU_BLOCK
+from . import kv8
 from .attn_desc import AttnDesc
 
 
@@ -146,6 +147,92 @@ def kv_move_slots(kv: torch.Tensor, src_slots: torch.Tensor, dst_slots: torch.Te
     dp, do = _slot_to_page(dst_slots, ps)
     vals = kv[:, sp, :, :, so].clone()  # [L, n, 2, Hkv, hd]
     kv[:, dp, :, :, do] = vals
+
+
+# ------------------------------------------------------- 8-bit KV cache
+# The rules of the cache (scales, page starts, repeated slots) are those of ``ops.kv8``.
+def rope_qkv_append8(
+    qkv: torch.Tensor,
+    table: torch.Tensor,
+    positions: torch.Tensor,
+    slots: torch.Tensor,
+    kv_layer: kv8.Kv8Layer,
+    num_heads: int,
+    num_kv_heads: int,
+    out_dtype: torch.dtype | None = None,
+) -> torch.Tensor:
+    """Rotate q/k, write k and v into the 8-bit cache at ``slots``; return rotated q [M, Hq, hd]."""
+    m = qkv.shape[0]
+    hd = kv_layer.data.shape[-1]
+    x = qkv.float().reshape(m, num_heads + 2 * num_kv_heads, hd)
+    if m and not bool(((positions >= 0) & (positions < table.shape[0])).all()):
+        raise IndexError(f"position outside the rotary table of {table.shape[0]}")
+    cs = table[positions.long()]
+    cos, sin = cs[:, None, : hd // 2], cs[:, None, hd // 2:]
+    a, b = x[..., : hd // 2], x[..., hd // 2:]
+    rot = torch.cat((a * cos - b * sin, b * cos + a * sin), dim=-1)
+    rows = torch.stack((rot[:, num_heads: num_heads + num_kv_heads], x[:, num_heads + num_kv_heads:]), dim=1)[:, None]
+    if m:
+        kv8.write_rows(kv_layer.data[None], kv_layer.scale[None], rows, kv8.needed_scale(rows.abs().amax(-1)), slots)
+    return rot[:, :num_heads].to(out_dtype or qkv.dtype)
+
+
+def attention8(q: torch.Tensor, kv_layer: kv8.Kv8Layer, desc: AttnDesc, scale: float | None = None) -> torch.Tensor:
+    """``attention`` over one layer of the 8-bit cache; a row that sees no key answers zero."""
+    return attention(q, kv_layer.values(), desc, scale)
+
+
+def attention8_causal(q: torch.Tensor, kv_layer: kv8.Kv8Layer, desc: AttnDesc, causal_start: int,
+                      scale: float | None = None) -> torch.Tensor:
+    """``attention8`` of a chunk at positions ``causal_start ..`` whose own keys are in the cache already."""
+    m = q.shape[0]
+    limit = torch.arange(causal_start + 1, causal_start + m + 1, dtype=torch.int32, device=q.device)
+    return attention8(q, kv_layer, AttnDesc(desc.prefix_pages, int(desc.prefix_pages.numel()), int(causal_start), 0,
+                                            limit, limit, desc.row_mask, desc.tail_pages), scale)
+
+
+def kv8_copy_pages(cache: kv8.Kv8Cache, copies: torch.Tensor) -> None:
+    """For each (src page, dst page, ntok): dst gets the first ntok slots and the scale of src in every layer,
+    zeros behind them; with ntok 0 it becomes an empty page.  A destination may appear once only, and not as a
+    source."""
+    plan = copies.tolist()
+    pages, ps = cache.data.shape[1], cache.data.shape[-2]
+    used = [s for s, _, _ in plan] + [d for _, d, _ in plan]
+    for src, dst, n in plan:
+        if not (0 <= src < pages and 0 <= dst < pages and 0 <= n <= ps):
+            raise IndexError(f"page copy ({src}, {dst}, {n}) is outside the cache of {pages} pages of {ps} slots")
+        if used.count(dst) != 1:
+            raise IndexError(f"page {dst} is a destination of one copy and named by another")
+    data = cache.data.view(torch.uint8)
+    for src, dst, n in plan:
+        data[:, dst, :, :, :n] = data[:, src, :, :, :n]
+        data[:, dst, :, :, n:] = 0
+        cache.scale[:, dst] = cache.scale[:, src] if n else 0.0
+
+
+def kv8_move_slots(cache: kv8.Kv8Cache, src_slots: torch.Tensor, dst_slots: torch.Tensor) -> None:
+    """Move slot contents (all layers, k and v); sources are read before any write.  A row needs its source
+    page's scale."""
+    pages, ps = cache.data.shape[1], cache.data.shape[-2]
+    if src_slots.numel() and not bool(((src_slots >= 0) & (src_slots < pages * ps)).all()):
+        raise IndexError(f"source slot outside the cache of {pages} pages of {ps} slots")
+    sp, so = _slot_to_page(src_slots, ps)
+    need = cache.scale[:, sp].transpose(0, 1)  # [n, layers, 2, kv_heads]
+    rows = cache.data.view(torch.uint8)[:, sp, :, :, so].view(torch.float8_e4m3fn).float() * need[..., None]
+    kv8.write_rows(cache.data, cache.scale, rows, need, dst_slots)
+
+
+def kv8_read_pages(cache: kv8.Kv8Cache | kv8.Kv8Layer, pages: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """The values of ``pages``: [n, 2, kv_heads, page_size, hd] of a layer, [layers, n, ...] of a cache (held to the
+    largest finite value of ``dtype``)."""
+    idx = pages.long()
+    data, scale = cache.data.view(torch.uint8), cache.scale
+    if data.dim() == 6:
+        data, scale = data[:, idx], scale[:, idx]
+    else:
+        data, scale = data[idx], scale[idx]
+    lim = torch.finfo(dtype).max
+    return (data.view(torch.float8_e4m3fn).float() * scale[..., None, None]).clamp(-lim, lim).to(dtype)
 
 
 def topk_logprobs(logits: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:

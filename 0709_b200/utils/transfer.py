@@ -35,6 +35,7 @@ ERROR_NAMES = {
     2: "index out of range",
     3: "unsupported configuration",
     4: "peer rank did not deliver its partial in time",
+    5: "value that the 8-bit KV cache cannot hold (NaN, infinite or too large)",
 }
 
 
