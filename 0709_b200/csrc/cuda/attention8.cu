@@ -123,27 +123,396 @@ __device__ __forceinline__ void load_q4(const Attn8Params& p, int64_t pair, int 
   for (int i = 0; i < 4; ++i) q[i] = to_f32(e[i]);
 }
 
-// One warp per (row, q head) and split over the shared keys.
-template <typename T>
-__global__ void __launch_bounds__(128) attn8_split_kernel(Attn8Params p) {
+// ------------------------------------------------------------ split pass
+// Four codes (one 32-bit word) as fp16: code = 256 * value.  An e4m3 byte moved to the top of a
+// half and shifted right by one under its sign is the fp16 number code / 256, subnormals included,
+// so two masks convert a pair; the factor joins the scales.
+__device__ __forceinline__ uint32_t half_pair(uint32_t v) { return (v & 0x80008000u) | ((v >> 1) & 0x3f803f80u); }
+
+__device__ __forceinline__ void mma16816(float* c, const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Visibility of keys x0 .. x0 + 15 to a row, one bit each.
+__device__ __forceinline__ uint32_t visible16(const Attn8Params& p, int m, int x0, int full, int len, int mask_base) {
+  const int nf = min(max(full - x0, 0), 16);
+  uint32_t v = (1u << nf) - 1u;
+  if (x0 + 16 > full && full < len) {
+    for (int j = nf; j < 16; ++j)
+      if (attn8_visible(p, m, x0 + j, full, len, mask_base)) v |= 1u << j;
+  }
+  return v;
+}
+
+template <int MT>
+struct SplitCfg {
+  static constexpr int kWarps = 8;
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kStages = MT == 1 ? 3 : 6;
+  static constexpr int kUnitBytes = 4096;  // 16 keys: K 2 KB, V 2 KB
+  static constexpr int kRingBytes = kWarps * kStages * kUnitBytes;
+  static constexpr int kQBytes = MT * 8 * 512;
+  static constexpr int kMergeBytes = kWarps * kRows * kHd * 4;
+  static_assert(kMergeBytes <= kRingBytes, "the warps' partial rows reuse the ring");
+  static constexpr int kSmem = 1024 + kRingBytes + kQBytes + kRows * 4 + kWarps * kRows * 8 + kWarps * kStages * 8;
+};
+
+// One CTA per (kv head, split of the shared keys, tile of 16 MT query rows); query rows are
+// (row, head of the group) pairs.  Each warp streams its own units of 16 keys (K and V of one head:
+// 4 KB by TMA, 128B-swizzled) through a private ring, so no warp waits for another before the final
+// merge; a warp holds all the tile's rows: S = Q K^T and O += P V on m16n8k16 tensor-core
+// instructions whose operands are converted from the codes in registers.  With few rows the pass is
+// bound by the cache's bytes; going through registers costs the shared memory one write and one read
+// of the codes and nothing else, where a TMEM pipeline would have to write both operands back in fp16.
+template <typename T, int MT>
+__global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
+    attn8_split_kernel(const __grid_constant__ CUtensorMap map, Attn8Params p) {
+  using C = SplitCfg<MT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem;
+  uint8_t* q_s = ring + C::kRingBytes;                       // A fragments [MT][8 k-steps][32 lanes] x 16 B
+  float* rowfac = reinterpret_cast<float*>(q_s + C::kQBytes);  // [rows]: scores per unit of Q K (log2 units)
+  float2* ml_s = reinterpret_cast<float2*>(rowfac + C::kRows);  // [warps][rows]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ml_s + C::kWarps * C::kRows);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int h = blockIdx.x, split = blockIdx.y;
+  const int G = p.Hq / p.Hkv;
+  const int rows_total = p.M * G;
+  const int tile0 = blockIdx.z * C::kRows;
+  uint64_t* bar = bars + warp * C::kStages;
+  if (lane == 0) {
+    for (int s = 0; s < C::kStages; ++s) mbar_init(&bar[s], 1);
+    fence_barrier_init();
+  }
+  if (tid == 0) tma_prefetch_desc(&map);
+  __syncwarp();
   pdl_wait();
   pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
-  const int64_t pair = static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  if (pair >= pairs) return;
-  const int m = static_cast<int>(pair / p.Hq), hq = static_cast<int>(pair % p.Hq);
-  const Attn8Shape s = attn8_shape(p);
-  const int len = p.row_len[m], full = min(p.row_full[m], len);
-  const int end = min(s.shared_end, len);
-  const int per = (((s.shared_end + p.splits - 1) / p.splits) + 31) & ~31;
-  const int x0 = blockIdx.y * per;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, ref = -INFINITY, l = 0.f;
-  load_q4<T>(p, pair, lane, q);
-  fold_keys8<false>(p, s, m, hq / (p.Hq / p.Hkv), lane, q, x0, min(end, x0 + per), full, len, ref, l, o);
-  const int64_t rec = blockIdx.y * pairs + pair;
-  if (lane == 0) p.part_ml[rec] = make_float2(ref, l);
-  *reinterpret_cast<float4*>(p.part_o + rec * kHd + lane * 4) = make_float4(o[0], o[1], o[2], o[3]);
+  const Attn8Shape sh = attn8_shape(p);
+
+  // The tile's limits: last visible key of any row, first key that some row may not see.
+  int len_max = 0, full_min = 0x7fffffff;
+  if (lane < C::kRows && tile0 + lane < rows_total) {
+    const int m = (tile0 + lane) / G;
+    len_max = p.row_len[m];
+    full_min = min(p.row_full[m], len_max);
+  }
+  len_max = __reduce_max_sync(0xffffffffu, len_max);
+  full_min = __reduce_min_sync(0xffffffffu, full_min);
+  const int end = min(sh.shared_end, len_max);
+  const int units = (end + 15) >> 4;
+  const int per = max((units + p.splits - 1) / p.splits, C::kWarps);
+  const int u0 = split * per;
+  const int mine = max(0, (min(units, u0 + per) - u0 - warp + C::kWarps - 1) / C::kWarps);  // units of this warp
+
+  // Lane i: page and scales of this warp's unit base + i (two pages when a page has 8 slots).
+  const int ps = 1 << p.page_shift;
+  const bool two = p.page_shift == 3;
+  struct Window {
+    int page[2];
+    float ks[2], vs[2];
+  };
+  auto load_window = [&](int base) {
+    Window w;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      w.page[e] = 0;
+      w.ks[e] = 0.f;
+      w.vs[e] = 1.f;
+      const int x = ((u0 + warp + (base + lane) * C::kWarps) << 4) + e * 8;
+      if (base + lane < mine && x < end && (e == 0 || two)) {
+        const int j = x >> p.page_shift;
+        const int page = j < p.n_prefix ? p.prefix_pages[j] : -1;
+        if (page < 0 || page >= p.num_pages) {
+          set_error(p.err, kErrBadIndex);
+        } else {
+          const int64_t ph = static_cast<int64_t>(page) * 2 * p.Hkv + h;
+          w.page[e] = page;
+          w.ks[e] = p.scale[ph];
+          const float v = p.scale[ph + p.Hkv];
+          if (v > 0.f) w.vs[e] = v;
+        }
+      }
+    }
+    if (!two) {
+      w.ks[1] = w.ks[0];
+      w.vs[1] = w.vs[0];
+    }
+    return w;
+  };
+  Window cur = load_window(0), nxt = load_window(32);
+  int window = 0;  // first unit of cur
+
+  uint8_t* my_ring = ring + warp * C::kStages * C::kUnitBytes;
+  auto issue = [&](int i) {  // whole warp: unit i of this warp into its stage
+    const int w = i - window;
+    const int pa = __shfl_sync(0xffffffffu, w < 32 ? cur.page[0] : nxt.page[0], w & 31);
+    const int pb = two ? __shfl_sync(0xffffffffu, w < 32 ? cur.page[1] : nxt.page[1], w & 31) : 0;
+    if (lane == 0) {
+      const int s = i % C::kStages;
+      uint8_t* dst = my_ring + s * C::kUnitBytes;
+      const int off = ((u0 + warp + i * C::kWarps) << 4) & (ps - 1);
+      mbar_arrive_expect_tx(&bar[s], C::kUnitBytes);
+      const int yk = ((pa * 2) * p.Hkv + h) * ps + off, yv = yk + p.Hkv * ps;
+      tma_load_2d(dst, &map, &bar[s], 0, yk);
+      tma_load_2d(dst + 2048, &map, &bar[s], 0, yv);
+      if (two) {
+        const int zk = ((pb * 2) * p.Hkv + h) * ps;
+        tma_load_2d(dst + 1024, &map, &bar[s], 0, zk);
+        tma_load_2d(dst + 3072, &map, &bar[s], 0, zk + p.Hkv * ps);
+      }
+    }
+  };
+  const int ahead = min(mine, C::kStages);
+  for (int i = 0; i < ahead; ++i) issue(i);
+
+  // Q rows as fp16 A fragments, each row scaled by a power of two so that its largest element is in
+  // [1, 2): bf16 rows of any size fit.  Dimension 16 (2 t + s) + 4 i + b of a row belongs to k-step
+  // 4 s + i of the lanes t: bytes b of the K word that these lanes convert.
+  for (int r = warp; r < C::kRows; r += C::kWarps) {
+    float q[4] = {0.f, 0.f, 0.f, 0.f};
+    const int grow = tile0 + r;
+    if (grow < rows_total)
+      load_q4<T>(p, static_cast<int64_t>(grow / G) * p.Hq + h * G + grow % G, lane, q);
+    uint32_t ab = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ab = max(ab, __float_as_uint(q[e]) & 0x7fffffffu);
+    ab = __reduce_max_sync(0xffffffffu, ab);
+    int e2 = static_cast<int>(ab >> 23) - 127;
+    if (ab == 0 || ab >= 0x7f800000u) e2 = 0;
+    e2 = min(max(e2, -126), 126);
+    const float down = __int_as_float((127 - e2) << 23);
+    const int c = lane >> 2, ks = (c & 1) * 4 + (lane & 3);
+    const int hi = (r >> 3) & 1;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(q_s) + (((r >> 4) * 8 + ks) * 32 + (r & 7) * 4 + (c >> 1)) * 4;
+    dst[hi] = pack_half2(q[0] * down, q[2] * down);
+    dst[2 + hi] = pack_half2(q[1] * down, q[3] * down);
+    if (lane == 0) rowfac[r] = p.scale_log2 * __int_as_float((127 + e2) << 23) * 256.f;
+  }
+  __syncthreads();
+
+  float o[MT][16][4];
+  float ref[MT][2], sum[MT][2], fac[MT][2];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[mt][j][e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      ref[mt][e] = -INFINITY;
+      sum[mt][e] = 0.f;
+      fac[mt][e] = rowfac[mt * 16 + e * 8 + g];
+    }
+  }
+
+  bool ok = true;
+  for (int i = 0; i < mine && ok; ++i) {
+    if (i - window == 32) {
+      window += 32;
+      cur = nxt;
+      nxt = load_window(window + 32);
+    }
+    const int stage = i % C::kStages;
+    ok = mbar_wait(&bar[stage], (i / C::kStages) & 1, p.err);
+    const uint8_t* kb = my_ring + stage * C::kUnitBytes;
+    const uint8_t* vb = kb + 2048;
+    // S: lanes 4 g + t hold keys 8 nt + 2 t, + 1 of rows g and g + 8.
+    float s[MT][2][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][nt][e] = 0.f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint4 kw[2];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+        kw[nt] = *reinterpret_cast<const uint4*>(kb + sw128_offset(nt * 8 + g, 2 * t + half));
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint4 a[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          a[mt] = *reinterpret_cast<const uint4*>(q_s + ((mt * 8 + half * 4 + w) * 32 + lane) * 16);
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const uint32_t x = w == 0 ? kw[nt].x : w == 1 ? kw[nt].y : w == 2 ? kw[nt].z : kw[nt].w;
+          const uint32_t b0 = half_pair(x << 8), b1 = half_pair(x);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) mma16816(s[mt][nt], a[mt], b0, b1);
+        }
+      }
+    }
+    // u = score * log2(e) + log2(v scale); P = 2^(u - ref).
+    const int wl = (i - window) & 31;
+    float kf[2], lv[2], iv[2];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      kf[nt] = __shfl_sync(0xffffffffu, cur.ks[nt], wl);
+      const float v = __shfl_sync(0xffffffffu, cur.vs[nt], wl);
+      const int ev = static_cast<int>(__float_as_uint(v) >> 23) - 127;
+      lv[nt] = static_cast<float>(ev);
+      iv[nt] = __int_as_float((127 - ev) << 23);
+    }
+    const int x0 = (u0 + warp + i * C::kWarps) << 4;
+    const bool masked = x0 + 16 > min(full_min, end);
+    uint4 pa[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t vis = 0xffffu;
+        if (masked) {
+          const int grow = tile0 + mt * 16 + e * 8 + g;
+          vis = 0;
+          if (grow < rows_total) {
+            const int m = grow / G;
+            const int len = min(p.row_len[m], end);
+            vis = visible16(p, m, x0, min(p.row_full[m], len), len, sh.mask_base);
+          }
+        }
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float& u = s[mt][nt][e * 2 + k];
+            u = fmaf(u, fac[mt][e] * kf[nt], lv[nt]);
+            if (!((vis >> (nt * 8 + 2 * t + k)) & 1u)) u = -INFINITY;
+            top[e] = fmaxf(top[e], u);
+          }
+      }
+      // ref follows the row's largest u only when that grew by more than 8 (a factor of 256): P stays
+      // far inside fp16, and O is rarely rescaled.
+      if (__any_sync(0xffffffffu, top[0] > ref[mt][0] + 8.f || top[1] > ref[mt][1] + 8.f)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          if (mx > ref[mt][e] + 8.f) {
+            const float a = ref[mt][e] > -INFINITY ? ex2(ref[mt][e] - mx) : 0.f;
+            ref[mt][e] = mx;
+            sum[mt][e] *= a;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              o[mt][j][e * 2] *= a;
+              o[mt][j][e * 2 + 1] *= a;
+            }
+          }
+        }
+      }
+      uint32_t packed[2][2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float neg = ref[mt][e] > -INFINITY ? -ref[mt][e] : 0.f;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          const float p0 = ex2(s[mt][nt][e * 2] + neg), p1 = ex2(s[mt][nt][e * 2 + 1] + neg);
+          sum[mt][e] = fmaf(p0 + p1, iv[nt], sum[mt][e]);
+          packed[nt][e] = pack_half2(p0, p1);
+        }
+      }
+      pa[mt] = make_uint4(packed[0][0], packed[0][1], packed[1][0], packed[1][1]);
+    }
+    // O += P V: lane (g, t) converts dimensions 16 g .. 16 g + 15 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+    uint4 v4[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      v4[k] = *reinterpret_cast<const uint4*>(vb + sw128_offset(2 * t + (k & 1) + (k >> 1) * 8, g));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = w == 0 ? v4[k].x : w == 1 ? v4[k].y : w == 2 ? v4[k].z : v4[k].w;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const uint32_t sel = static_cast<uint32_t>(b << 4 | (4 + b) << 12);
+        const uint32_t b0 = half_pair(__byte_perm(x[0], x[1], sel)), b1 = half_pair(__byte_perm(x[2], x[3], sel));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][w * 4 + b], pa[mt], b0, b1);
+      }
+    }
+    __syncwarp();  // the stage is read: it may be filled again
+    if (i + C::kStages < mine) issue(i + C::kStages);
+  }
+
+  // Merge the warps: (ref, sum) per row, then O over the drained rings.  Lane (g, t) holds
+  // dimensions 32 t .. 32 t + 31 of rows g and g + 8; float4 f of a row lands at f ^ (2 t + (g & 1)).
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float l = sum[mt][e];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (t == 0) ml_s[warp * C::kRows + mt * 16 + e * 8 + g] = make_float2(ref[mt][e], l);
+    }
+  __syncthreads();  // every warp is done with its ring
+  float* o_s = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float* row = o_s + (warp * C::kRows + mt * 16 + e * 8 + g) * kHd;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // c registers 2 e + k of n-tile j: dimension 32 t + 16 k + j
+        const int k = i >> 2, j = (i & 3) * 4;
+        *reinterpret_cast<float4*>(row + (t * 8 + (i ^ (2 * t + (g & 1)))) * 4) =
+            make_float4(o[mt][j][e * 2 + k], o[mt][j + 1][e * 2 + k], o[mt][j + 2][e * 2 + k], o[mt][j + 3][e * 2 + k]);
+      }
+    }
+  __syncthreads();
+  for (int it = tid; it < C::kRows * 32; it += 256) {
+    const int r = it >> 5, f = it & 31;  // one warp per row
+    const int grow = tile0 + r;
+    if (grow >= rows_total) continue;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < C::kWarps) ml = ml_s[lane * C::kRows + r];
+    if (ml.y == 0.f) ml.x = -INFINITY;
+    const float mx = warp_max(ml.x);
+    // A NaN sum keeps its weight so that it shows in the result.
+    const float w = ml.y == 0.f ? 0.f : mx > -INFINITY ? ex2(ml.x - mx) : 1.f;
+    const float l = warp_sum(ml.y == 0.f ? 0.f : w * ml.y);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int at = (f & ~7) + ((f & 7) ^ (2 * (f >> 3) + (r & 1)));
+#pragma unroll
+    for (int k = 0; k < C::kWarps; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k) * 256.f;
+      const float4 v = *reinterpret_cast<const float4*>(o_s + (k * C::kRows + r) * kHd + at * 4);
+      if (wk != 0.f) {
+        acc.x = fmaf(wk, v.x, acc.x);
+        acc.y = fmaf(wk, v.y, acc.y);
+        acc.z = fmaf(wk, v.z, acc.z);
+        acc.w = fmaf(wk, v.w, acc.w);
+      }
+    }
+    const int64_t rec = (static_cast<int64_t>(split) * p.M + grow / G) * p.Hq + h * G + grow % G;
+    if (f == 0) p.part_ml[rec] = make_float2(mx, l);
+    if (l != 0.f) *reinterpret_cast<float4*>(p.part_o + rec * kHd + f * 4) = acc;
+  }
 }
 
 // One warp per (row, q head): the row's private tail keys, then the splits' records in split order
@@ -186,19 +555,30 @@ __global__ void __launch_bounds__(128) attn8_merge_kernel(Attn8Params p) {
   *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + pair * kHd + lane * 4) = *reinterpret_cast<const uint2*>(v);
 }
 
+template <typename T, int MT>
+static cudaError_t launch_split8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
+  constexpr int smem = SplitCfg<MT>::kSmem;
+  const cudaError_t e =
+      cudaFuncSetAttribute(attn8_split_kernel<T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  const int rows = p.M * (p.Hq / p.Hkv);
+  const dim3 grid(p.Hkv, p.splits, (rows + 16 * MT - 1) / (16 * MT));
+  return launch_k(attn8_split_kernel<T, MT>, grid, dim3(256), smem, st, map, p);
+}
+
 template <typename T>
-static cudaError_t launch_typed8(const Attn8Params& p, cudaStream_t st) {
-  const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.M) * p.Hq + 3) / 4);
+static cudaError_t launch_typed8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
   if (p.splits > 0) {
-    const cudaError_t e = launch_k(attn8_split_kernel<T>, dim3(blocks, p.splits), dim3(128), 0, st, p);
+    const cudaError_t e = p.row_tile == 16 ? launch_split8<T, 1>(map, p, st) : launch_split8<T, 2>(map, p, st);
     if (e != cudaSuccess) return e;
   }
+  const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.M) * p.Hq + 3) / 4);
   return launch_k(attn8_merge_kernel<T>, dim3(blocks), dim3(128), 0, st, p);
 }
 
-cudaError_t launch_attention8(const CUtensorMap&, const Attn8Params& p, cudaStream_t st) {
+cudaError_t launch_attention8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
   if (p.M == 0) return cudaSuccess;
-  return p.bf16 ? launch_typed8<__nv_bfloat16>(p, st) : launch_typed8<__half>(p, st);
+  return p.bf16 ? launch_typed8<__nv_bfloat16>(map, p, st) : launch_typed8<__half>(map, p, st);
 }
 
 }  // namespace atlas

@@ -805,6 +805,11 @@ void gather_logprobs(torch::Tensor logits, torch::Tensor rows, torch::Tensor tok
 
 }  // namespace
 
+CUtensorMap map_kv8(const torch::Tensor& data) {
+  const int64_t rows = data.numel() / 128;
+  return map_2d(data, 128, rows, 128, static_cast<int>(std::min<int64_t>(data.size(-2), 16)));
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "sm_100a kernels: tcgen05/TMA GEMM and paged attention, fused norm/rope/append, KV copies, top-k";
   m.def("gemm", &gemm, "tcgen05 GEMM out = epi(x @ w^T); returns [bn, splits, kb_per_split]");

@@ -149,9 +149,17 @@ torch::Tensor kv8_read_pages(torch::Tensor data, torch::Tensor scale, torch::Ten
   return out;
 }
 
-// Splits of the shared keys: enough CTAs to fill the device, at least 128 keys each, 64 at most.
-int64_t pick_splits8(int64_t tiles, int64_t keys, int sms) {
-  return std::max<int64_t>(1, std::min<int64_t>({64, sms / std::max<int64_t>(tiles, 1), (keys + 127) / 128}));
+// The split pass's launch shape.  Rows of a kv head (query rows times group) go in tiles of 16 while
+// they fit one tile, else of 32; the splits fill the CTA slots (two per SM for the small tile), each
+// of at least 128 keys.
+struct Shape8 {
+  int row_tile, splits;
+};
+Shape8 pick_shape8(int64_t rows, int64_t Hkv, int64_t keys, int sms) {
+  const int tile = rows <= 16 ? 16 : 32;
+  const int64_t slots = static_cast<int64_t>(sms) * (tile == 16 ? 2 : 1);
+  const int64_t ctas = Hkv * ((rows + tile - 1) / tile);
+  return {tile, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, slots / ctas, (keys + 127) / 128})))};
 }
 
 std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data, torch::Tensor scale, c10::optional<torch::Tensor> dparams,
@@ -212,15 +220,21 @@ std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data
   p.scale_log2 = static_cast<float>(softmax_scale * kLog2e);
   // A captured call is sized for the longest context its graph may see (max_keys), an eager one for its own.
   const int64_t keys = std::max<int64_t>({shared_len, n_shared_pages << shift, max_keys});
-  p.splits = static_cast<int>(
-      keys > 0 || dparams.has_value() ? pick_splits8(Hkv, keys, at::cuda::getCurrentDeviceProperties()->multiProcessorCount) : 0);
+  CUtensorMap map{};
+  if (keys > 0 || dparams.has_value()) {
+    const Shape8 shape =
+        pick_shape8(M * (Hq / Hkv), Hkv, keys, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
+    p.row_tile = shape.row_tile;
+    p.splits = shape.splits;
+    map = map_kv8(data);
+  }
   torch::Tensor parts;
   if (p.splits > 0) {
     parts = torch::empty({p.splits * M * Hq * 130}, q.options().dtype(torch::kFloat32));
     p.part_o = parts.data_ptr<float>();
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<int64_t>(p.splits) * M * Hq * 128);
   }
-  check_launch(atlas::launch_attention8(CUtensorMap{}, p, at::cuda::getCurrentCUDAStream()), "attention8");
+  check_launch(atlas::launch_attention8(map, p, at::cuda::getCurrentCUDAStream()), "attention8");
   return {out, p.splits > 0 ? 2 : 1};
 }
 

@@ -58,8 +58,10 @@ struct Attn8Params {
   int* err;
   int M, Hq, Hkv, page_shift, num_pages, n_prefix;
   int mask_words, tail_stride, splits, bf16;
+  int row_tile;  // query rows of a kv head per CTA of the split pass: 16 or 32
   float scale_log2;  // softmax scale * log2(e)
 };
+// map: the layer as rows of 128 bytes, box (128, min(page size, 16)), 128B swizzle.
 cudaError_t launch_attention8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st);
 
 }  // namespace atlas
