@@ -124,10 +124,17 @@ __device__ __forceinline__ void load_q4(const Attn8Params& p, int64_t pair, int 
 }
 
 // ------------------------------------------------------------ split pass
-// Four codes (one 32-bit word) as fp16: code = 256 * value.  An e4m3 byte moved to the top of a
-// half and shifted right by one under its sign is the fp16 number code / 256, subnormals included,
-// so two masks convert a pair; the factor joins the scales.
-__device__ __forceinline__ uint32_t half_pair(uint32_t v) { return (v & 0x80008000u) | ((v >> 1) & 0x3f803f80u); }
+// The two codes in the low (high) half of w as fp16 values.
+__device__ __forceinline__ uint32_t half_pair_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t half_pair_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
 
 __device__ __forceinline__ void mma16816(float* c, const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -285,8 +292,8 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
   for (int i = 0; i < ahead; ++i) issue(i);
 
   // Q rows as fp16 A fragments, each row scaled by a power of two so that its largest element is in
-  // [1, 2): bf16 rows of any size fit.  Dimension 16 (2 t + s) + 4 i + b of a row belongs to k-step
-  // 4 s + i of the lanes t: bytes b of the K word that these lanes convert.
+  // [1, 2): bf16 rows of any size fit.  Dimensions 16 (2 t + s) + 4 i .. + 3 of a row belong to k-step
+  // 4 s + i of the lanes t: the bytes of the K word that these lanes convert.
   for (int r = warp; r < C::kRows; r += C::kWarps) {
     float q[4] = {0.f, 0.f, 0.f, 0.f};
     const int grow = tile0 + r;
@@ -303,9 +310,9 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
     const int c = lane >> 2, ks = (c & 1) * 4 + (lane & 3);
     const int hi = (r >> 3) & 1;
     uint32_t* dst = reinterpret_cast<uint32_t*>(q_s) + (((r >> 4) * 8 + ks) * 32 + (r & 7) * 4 + (c >> 1)) * 4;
-    dst[hi] = pack_half2(q[0] * down, q[2] * down);
-    dst[2 + hi] = pack_half2(q[1] * down, q[3] * down);
-    if (lane == 0) rowfac[r] = p.scale_log2 * __int_as_float((127 + e2) << 23) * 256.f;
+    dst[hi] = pack_half2(q[0] * down, q[1] * down);
+    dst[2 + hi] = pack_half2(q[2] * down, q[3] * down);
+    if (lane == 0) rowfac[r] = p.scale_log2 * __int_as_float((127 + e2) << 23);
   }
   __syncthreads();
 
@@ -359,7 +366,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) {
           const uint32_t x = w == 0 ? kw[nt].x : w == 1 ? kw[nt].y : w == 2 ? kw[nt].z : kw[nt].w;
-          const uint32_t b0 = half_pair(x << 8), b1 = half_pair(x);
+          const uint32_t b0 = half_pair_lo(x), b1 = half_pair_hi(x);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) mma16816(s[mt][nt], a[mt], b0, b1);
         }
@@ -384,25 +391,25 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        uint32_t vis = 0xffffu;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) s[mt][nt][e * 2 + k] = fmaf(s[mt][nt][e * 2 + k], fac[mt][e] * kf[nt], lv[nt]);
         if (masked) {
           const int grow = tile0 + mt * 16 + e * 8 + g;
-          vis = 0;
+          uint32_t vis = 0;
           if (grow < rows_total) {
             const int m = grow / G;
             const int len = min(p.row_len[m], end);
             vis = visible16(p, m, x0, min(p.row_full[m], len), len, sh.mask_base);
           }
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (!((vis >> (nt * 8 + 2 * t + k)) & 1u)) s[mt][nt][e * 2 + k] = -INFINITY;
         }
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            float& u = s[mt][nt][e * 2 + k];
-            u = fmaf(u, fac[mt][e] * kf[nt], lv[nt]);
-            if (!((vis >> (nt * 8 + 2 * t + k)) & 1u)) u = -INFINITY;
-            top[e] = fmaxf(top[e], u);
-          }
+        top[e] = fmaxf(fmaxf(s[mt][0][e * 2], s[mt][0][e * 2 + 1]), fmaxf(s[mt][1][e * 2], s[mt][1][e * 2 + 1]));
       }
       // ref follows the row's largest u only when that grew by more than 8 (a factor of 256): P stays
       // far inside fp16, and O is rarely rescaled.
@@ -447,11 +454,13 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[k] = w == 0 ? v4[k].x : w == 1 ? v4[k].y : w == 2 ? v4[k].z : v4[k].w;
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const uint32_t sel = static_cast<uint32_t>(b << 4 | (4 + b) << 12);
-        const uint32_t b0 = half_pair(__byte_perm(x[0], x[1], sel)), b1 = half_pair(__byte_perm(x[2], x[3], sel));
+      for (int b = 0; b < 4; b += 2) {  // codes b, b + 1 of both keys, one pair per dimension
+        const uint32_t sel = b == 0 ? 0x5140u : 0x7362u;
+        const uint32_t y0 = __byte_perm(x[0], x[1], sel), y1 = __byte_perm(x[2], x[3], sel);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][w * 4 + b], pa[mt], b0, b1);
+        for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][w * 4 + b], pa[mt], half_pair_lo(y0), half_pair_lo(y1));
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][w * 4 + b + 1], pa[mt], half_pair_hi(y0), half_pair_hi(y1));
       }
     }
     __syncwarp();  // the stage is read: it may be filled again
@@ -500,7 +509,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
     const int at = (f & ~7) + ((f & 7) ^ (2 * (f >> 3) + (r & 1)));
 #pragma unroll
     for (int k = 0; k < C::kWarps; ++k) {
-      const float wk = __shfl_sync(0xffffffffu, w, k) * 256.f;
+      const float wk = __shfl_sync(0xffffffffu, w, k);
       const float4 v = *reinterpret_cast<const float4*>(o_s + (k * C::kRows + r) * kHd + at * 4);
       if (wk != 0.f) {
         acc.x = fmaf(wk, v.x, acc.x);
