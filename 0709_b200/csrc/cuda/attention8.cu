@@ -11,37 +11,9 @@
 
 #include <cuda_fp8.h>
 
-#include "common.cuh"
-#include "kv8.h"
-#include "launch.h"
+#include "attention8.cuh"
 
 namespace atlas {
-
-namespace {
-constexpr int kHd = 128;
-}  // namespace
-
-struct Attn8Shape {
-  int shared_len, n_shared, mask_base, shared_end;
-};
-
-__device__ __forceinline__ Attn8Shape attn8_shape(const Attn8Params& p) {
-  Attn8Shape s;
-  const bool dev = p.dparams != nullptr;
-  s.shared_len = dev ? p.dparams[0] : p.shared_len;
-  s.n_shared = dev ? p.dparams[1] : p.n_shared_pages;
-  s.mask_base = dev ? p.dparams[2] : p.mask_base;
-  s.shared_end = max(s.n_shared << p.page_shift, s.shared_len);
-  return s;
-}
-
-__device__ __forceinline__ bool attn8_visible(const Attn8Params& p, int m, int x, int full, int len, int mask_base) {
-  if (x >= len) return false;
-  if (x < full) return true;
-  const int b = x - mask_base;
-  if (b < 0 || b >= 64 * p.mask_words) return false;
-  return (static_cast<uint64_t>(p.row_mask[static_cast<int64_t>(m) * p.mask_words + (b >> 6)]) >> (b & 63)) & 1ull;
-}
 
 __device__ __forceinline__ void decode4(uint32_t w, float* x) {
   const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xffff), __NV_E4M3);
@@ -124,46 +96,12 @@ __device__ __forceinline__ void load_q4(const Attn8Params& p, int64_t pair, int 
 }
 
 // ------------------------------------------------------------ split pass
-// The two codes in the low (high) half of w as fp16 values.
-__device__ __forceinline__ uint32_t half_pair_lo(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(w));
-  return r;
-}
-__device__ __forceinline__ uint32_t half_pair_hi(uint32_t w) {
-  uint32_t r;
-  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
-  return r;
-}
-
 __device__ __forceinline__ void mma16816(float* c, const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, "
       "%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// Visibility of keys x0 .. x0 + 15 to a row, one bit each.
-__device__ __forceinline__ uint32_t visible16(const Attn8Params& p, int m, int x0, int full, int len, int mask_base) {
-  const int nf = min(max(full - x0, 0), 16);
-  uint32_t v = (1u << nf) - 1u;
-  if (x0 + 16 > full && full < len) {
-    for (int j = nf; j < 16; ++j)
-      if (attn8_visible(p, m, x0 + j, full, len, mask_base)) v |= 1u << j;
-  }
-  return v;
 }
 
 template <int MT>
@@ -242,8 +180,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       w.page[e] = 0;
-      w.ks[e] = 0.f;
-      w.vs[e] = 1.f;
+      w.ks[e] = w.vs[e] = 1.f;
       const int x = ((u0 + warp + (base + lane) * C::kWarps) << 4) + e * 8;
       if (base + lane < mine && x < end && (e == 0 || two)) {
         const int j = x >> p.page_shift;
@@ -251,10 +188,10 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
         if (page < 0 || page >= p.num_pages) {
           set_error(p.err, kErrBadIndex);
         } else {
-          const int64_t ph = static_cast<int64_t>(page) * 2 * p.Hkv + h;
           w.page[e] = page;
-          w.ks[e] = p.scale[ph];
-          const float v = p.scale[ph + p.Hkv];
+          const int64_t ph = static_cast<int64_t>(page) * 2 * p.Hkv + h;
+          const float k = p.scale[ph], v = p.scale[ph + p.Hkv];
+          if (k > 0.f) w.ks[e] = k;
           if (v > 0.f) w.vs[e] = v;
         }
       }
@@ -303,9 +240,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
 #pragma unroll
     for (int e = 0; e < 4; ++e) ab = max(ab, __float_as_uint(q[e]) & 0x7fffffffu);
     ab = __reduce_max_sync(0xffffffffu, ab);
-    int e2 = static_cast<int>(ab >> 23) - 127;
-    if (ab == 0 || ab >= 0x7f800000u) e2 = 0;
-    e2 = min(max(e2, -126), 126);
+    const int e2 = row_exponent(ab);
     const float down = __int_as_float((127 - e2) << 23);
     const int c = lane >> 2, ks = (c & 1) * 4 + (lane & 3);
     const int hi = (r >> 3) & 1;
@@ -401,7 +336,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
           if (grow < rows_total) {
             const int m = grow / G;
             const int len = min(p.row_len[m], end);
-            vis = visible16(p, m, x0, min(p.row_full[m], len), len, sh.mask_base);
+            vis = static_cast<uint32_t>(visible64(p, m, x0, min(p.row_full[m], len), len, sh.mask_base));
           }
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt)
@@ -578,7 +513,9 @@ static cudaError_t launch_split8(const CUtensorMap& map, const Attn8Params& p, c
 template <typename T>
 static cudaError_t launch_typed8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
   if (p.splits > 0) {
-    const cudaError_t e = p.row_tile == 16 ? launch_split8<T, 1>(map, p, st) : launch_split8<T, 2>(map, p, st);
+    const cudaError_t e = p.row_tile == 0    ? launch_attention8_tc(map, p, st)
+                          : p.row_tile == 16 ? launch_split8<T, 1>(map, p, st)
+                                             : launch_split8<T, 2>(map, p, st);
     if (e != cudaSuccess) return e;
   }
   const unsigned blocks = static_cast<unsigned>((static_cast<int64_t>(p.M) * p.Hq + 3) / 4);

@@ -1,0 +1,89 @@
+// Device helpers shared by the attention kernels over the 8-bit KV cache.
+#pragma once
+
+#include "common.cuh"
+#include "kv8.h"
+#include "launch.h"
+
+namespace atlas {
+
+namespace {
+constexpr int kHd = 128;
+}  // namespace
+
+struct Attn8Shape {
+  int shared_len, n_shared, mask_base, shared_end;
+};
+
+__device__ __forceinline__ Attn8Shape attn8_shape(const Attn8Params& p) {
+  Attn8Shape s;
+  const bool dev = p.dparams != nullptr;
+  s.shared_len = dev ? p.dparams[0] : p.shared_len;
+  s.n_shared = dev ? p.dparams[1] : p.n_shared_pages;
+  s.mask_base = dev ? p.dparams[2] : p.mask_base;
+  s.shared_end = max(s.n_shared << p.page_shift, s.shared_len);
+  return s;
+}
+
+// Scales of a page and head as the kernels use them: k scale, log2(v scale), 1 / v scale.  An empty
+// page (scale 0) holds zero codes: any positive scale reads it right.
+__device__ __forceinline__ float4 attn8_scales(const Attn8Params& p, int64_t page_head) {
+  const float k = p.scale[page_head], v = p.scale[page_head + p.Hkv];
+  const int e = v > 0.f ? static_cast<int>(__float_as_uint(v) >> 23) - 127 : 0;
+  return make_float4(k > 0.f ? k : 1.f, static_cast<float>(e), __int_as_float((127 - e) << 23), 0.f);
+}
+
+__device__ __forceinline__ bool attn8_visible(const Attn8Params& p, int m, int x, int full, int len, int mask_base) {
+  if (x >= len) return false;
+  if (x < full) return true;
+  const int b = x - mask_base;
+  if (b < 0 || b >= 64 * p.mask_words) return false;
+  return (static_cast<uint64_t>(p.row_mask[static_cast<int64_t>(m) * p.mask_words + (b >> 6)]) >> (b & 63)) & 1ull;
+}
+
+// Visibility of keys x0 .. x0 + 63 to row m, one bit each: those below `full`, and the marked ones
+// below `len`.
+__device__ __forceinline__ uint64_t visible64(const Attn8Params& p, int m, int x0, int full, int len, int mask_base) {
+  auto first = [](int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; };
+  const uint64_t sure = first(full - x0), in = first(len - x0);
+  if (!(in & ~sure)) return sure & in;
+  const int off = x0 - mask_base;  // mask bit of key x0; words outside the mask are zero
+  const int w = off >> 6, b = off & 63;
+  const int64_t* words = p.row_mask + static_cast<int64_t>(m) * p.mask_words;
+  const uint64_t lo = w >= 0 && w < p.mask_words ? static_cast<uint64_t>(words[w]) : 0ull;
+  const uint64_t hi = w + 1 >= 0 && w + 1 < p.mask_words ? static_cast<uint64_t>(words[w + 1]) : 0ull;
+  const uint64_t marked = b ? (lo >> b) | (hi << (64 - b)) : lo;
+  return (sure | marked) & in;
+}
+
+// Power of two that brings a row's largest magnitude (given as bits) into [1, 2); 0 for rows of zeros
+// and rows that are not finite.
+__device__ __forceinline__ int row_exponent(uint32_t amax_bits) {
+  if (amax_bits == 0 || amax_bits >= 0x7f800000u) return 0;
+  return min(max(static_cast<int>(amax_bits >> 23) - 127, -126), 126);
+}
+
+// The two codes in the low (high) half of w as fp16 values.
+__device__ __forceinline__ uint32_t half_pair_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t half_pair_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+}  // namespace atlas

@@ -1,0 +1,402 @@
+// Paged attention over the 8-bit KV cache for many query rows: tcgen05 tiles of 128 rows.
+//
+// One CTA holds two tiles ("slots") of 128 query rows of one kv head: two different row tiles over
+// the same keys, or -- when one tile holds all rows -- the same rows over alternate 64-key chunks,
+// each slot then being a split of its own.  14 warps:
+//   0-7   softmax, one thread per query row (0-3 slot 0, 4-7 slot 1);
+//   8-11  converters: e4m3 codes of a chunk -> fp16 operand tiles in the 128B-swizzled layout;
+//   12    TMA producer: the chunk's pages (K and V codes) and their scales;
+//   13    MMA issuer.
+// Q stays in TMEM as the A operand of S = Q K^T, P replaces S in place (fp16) and is the A operand of
+// O += P V, so the shared memory carries per 64-key chunk the codes (16 KB written, 16 KB read), the
+// fp16 tiles (32 KB written) and their reads by the MMAs (16 KB per product), and nothing for Q and P.
+// A slot's next S waits for its P V; the other slot's products run meanwhile.
+//
+// TMEM columns: S/P of the slots 0-63, 64-127; O 128-255, 256-383; Q 384-447, 448-511.
+
+#include "attention8.cuh"
+
+namespace atlas {
+
+namespace {
+constexpr int kChunk = 64;
+constexpr int kStages8 = 4;                    // chunks of codes in flight
+constexpr int kStages16 = 3;                   // converted chunks
+constexpr int kBytes8 = kChunk * kHd * 2;      // K | V codes
+constexpr int kHalf16 = kChunk * 128;          // 64 keys x 64 dimensions of fp16
+constexpr int kBytes16 = 4 * kHalf16;          // K halves | V halves
+constexpr int kThreads = 448;
+constexpr int kSmem = 1024 + kStages8 * kBytes8 + kStages16 * kBytes16 + (kStages8 + kStages16) * 128 + 256;
+constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
+}  // namespace
+
+// D (+)= A(tmem) * B(smem).
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+      : "memory");
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn8_tc_kernel(const __grid_constant__ CUtensorMap map, Attn8Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring8 = smem;
+  uint8_t* ring16 = ring8 + kStages8 * kBytes8;
+  // Per 8 keys of a chunk: k scale, log2(v scale), 1 / v scale (8 x float4 would waste a quarter: two arrays).
+  float4* sc8 = reinterpret_cast<float4*>(ring16 + kStages16 * kBytes16);  // [kStages8][8]
+  float4* sc16 = sc8 + kStages8 * 8;                                       // [kStages16][8]
+  uint64_t* full8 = reinterpret_cast<uint64_t*>(sc16 + kStages16 * 8);
+  uint64_t* empty8 = full8 + kStages8;
+  uint64_t* full16 = empty8 + kStages8;
+  uint64_t* empty16 = full16 + kStages16;
+  uint64_t* s_full = empty16 + kStages16;  // [2]
+  uint64_t* p_full = s_full + 2;           // [2], 128 arrivals
+  uint64_t* pv_done = p_full + 2;          // [2]
+  uint64_t* q_full = pv_done + 2;          // 256 arrivals
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int h = blockIdx.x;
+  const int G = p.Hq / p.Hkv;
+  const int rows_total = p.M * G;
+  const bool ksplit = p.tc_ksplit != 0;
+  // The longest causal tiles are launched first, so that the short ones fill the last wave.
+  const int z = p.causal_start >= 0 ? static_cast<int>(gridDim.z - 1 - blockIdx.z) : static_cast<int>(blockIdx.z);
+  const int row0 = z * (ksplit ? 128 : 256);
+  const int rows_cta = min(rows_total - row0, ksplit ? 128 : 256);
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages8; ++s) {
+      mbar_init(&full8[s], 1);
+      mbar_init(&empty8[s], 128);
+    }
+    for (int s = 0; s < kStages16; ++s) {
+      mbar_init(&full16[s], 128);
+      mbar_init(&empty16[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 128);
+      mbar_init(&pv_done[s], 1);
+    }
+    mbar_init(q_full, 256);
+    fence_barrier_init();
+    tma_prefetch_desc(&map);
+  }
+  if (warp == 0) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();  // after this CTA's TMEM allocation
+
+  // This split's chunks: up to the last key that any row of the CTA may see.
+  const Attn8Shape sh = attn8_shape(p);
+  int len_max = 0;
+  if (p.causal_start >= 0) {
+    len_max = p.causal_start + (row0 + rows_cta - 1) / G + 1;
+  } else {
+    for (int m = row0 / G + lane; m <= (row0 + rows_cta - 1) / G; m += 32) len_max = max(len_max, p.row_len[m]);
+    len_max = __reduce_max_sync(0xffffffffu, len_max);
+  }
+  const int end = min(sh.shared_end, len_max);
+  const int chunks_all = (end + kChunk - 1) / kChunk;
+  const int per = (chunks_all + p.tc_splits - 1) / p.tc_splits;
+  const int c0 = static_cast<int>(blockIdx.y) * per;
+  const int chunks = max(0, min(chunks_all, c0 + per) - c0);
+  const int ps = 1 << p.page_shift;
+
+  if (warp == 12) {
+    // ---- producer: lane g < 8 resolves 8 keys of the chunk; lane i of the first 32 loads ahead nothing else
+    bool ok = true;
+    const int box = min(ps, 16);
+    for (int c = 0; c < chunks && ok; ++c) {
+      const int s = c % kStages8;
+      const int x = (c0 + c) * kChunk + (lane & 7) * 8;
+      int page = 0;
+      float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);
+      if (x < end) {
+        const int j = x >> p.page_shift;
+        page = j < p.n_prefix ? p.prefix_pages[j] : -1;
+        if (page < 0 || page >= p.num_pages) {
+          set_error(p.err, kErrBadIndex);
+          page = 0;
+        } else if (lane < 8) {
+          sc = attn8_scales(p, static_cast<int64_t>(page) * 2 * p.Hkv + h);
+        }
+      }
+      if (c >= kStages8) ok = mbar_wait(&empty8[s], ((c / kStages8) - 1) & 1, p.err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane < 8) sc8[s * 8 + lane] = sc;
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(&full8[s], kBytes8);
+      __syncwarp();
+      // Lane g issues the box that starts at its 8 keys (every other lane when a box holds 16).
+      if (lane < 8 && (box == 8 || (lane & 1) == 0)) {
+        const int y = (page * 2 * p.Hkv + h) * ps + (x & (ps - 1));
+        uint8_t* dst = ring8 + s * kBytes8 + lane * 8 * kHd;
+        tma_load_2d(dst, &map, &full8[s], 0, y);
+        tma_load_2d(dst + kBytes8 / 2, &map, &full8[s], 0, y + p.Hkv * ps);
+      }
+    }
+  } else if (warp >= 8 && warp < 12) {
+    // ---- converters: one 16-byte piece of codes (16 dimensions of a key) per thread and step
+    const int row = (tid - 256) >> 3, piece = tid & 7;  // rows row, row + 16, ..
+    bool ok = true;
+    for (int c = 0; c < chunks && ok; ++c) {
+      const int s = c % kStages8, d = c % kStages16;
+      ok = mbar_wait(&full8[s], (c / kStages8) & 1, p.err);
+      if (ok && c >= kStages16) ok = mbar_wait(&empty16[d], ((c / kStages16) - 1) & 1, p.err);
+      if (!ok) break;
+      if (tid - 256 < 8) sc16[d * 8 + tid - 256] = sc8[s * 8 + tid - 256];
+      const uint8_t* src = ring8 + s * kBytes8;
+      uint8_t* dst = ring16 + d * kBytes16;
+      uint4 w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)  // K rows, then V rows
+        w[i] = *reinterpret_cast<const uint4*>(src + (i >> 2) * (kBytes8 / 2) + sw128_offset(row + (i & 3) * 16, piece));
+      mbar_arrive(&empty8[s]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint4 lo, hi;
+        lo.x = half_pair_lo(w[i].x);
+        lo.y = half_pair_hi(w[i].x);
+        lo.z = half_pair_lo(w[i].y);
+        lo.w = half_pair_hi(w[i].y);
+        hi.x = half_pair_lo(w[i].z);
+        hi.y = half_pair_hi(w[i].z);
+        hi.z = half_pair_lo(w[i].w);
+        hi.w = half_pair_hi(w[i].w);
+        // Pieces p and p + 4 of a row meet the same banks (the two 64-dimension halves): they store
+        // their two 16-byte parts in opposite order.
+        const int flip = piece >> 2;
+        uint8_t* half = dst + (i >> 2) * 2 * kHalf16 + flip * kHalf16;
+        const int r = row + (i & 3) * 16, at = 2 * (piece & 3);
+        *reinterpret_cast<uint4*>(half + sw128_offset(r, at + flip)) = flip ? hi : lo;
+        *reinterpret_cast<uint4*>(half + sw128_offset(r, at + (flip ^ 1))) = flip ? lo : hi;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&full16[d]);
+    }
+  } else if (warp == 13) {
+    if (lane == 0 && chunks > 0) {
+      const uint32_t idesc_s = umma_idesc_f16(128, kChunk, false, false, false);
+      const uint32_t idesc_o = umma_idesc_f16(128, kHd, false, false, true);
+      const int n0 = ksplit ? (chunks + 1) / 2 : chunks, n1 = ksplit ? chunks / 2 : chunks;
+      bool ok = mbar_wait(q_full, 0, p.err);
+      tc_fence_after();
+      auto issue_s = [&](int slot, int k) {
+        const int c = ksplit ? 2 * k + slot : k;
+        const int d = c % kStages16;
+        ok = ok && mbar_wait(&full16[d], (c / kStages16) & 1, p.err);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t kb = smem_u32(ring16 + d * kBytes16);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_f16_ts(tmem + slot * 64, tmem + 384 + slot * 64 + kk * 8,
+                      umma_desc_sw128(kb + (kk >> 2) * kHalf16 + (kk & 3) * 32, 16, 1024), idesc_s, kk > 0);
+        umma_commit(&s_full[slot]);
+      };
+      auto issue_pv = [&](int slot, int k) {
+        const int c = ksplit ? 2 * k + slot : k;
+        const int d = c % kStages16;
+        ok = ok && mbar_wait(&p_full[slot], k & 1, p.err);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t vb = smem_u32(ring16 + d * kBytes16) + 2 * kHalf16;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          umma_f16_ts(tmem + 128 + slot * 128, tmem + slot * 64 + kk * 8, umma_desc_sw128(vb + kk * 2048, kHalf16, 1024),
+                      idesc_o, (k > 0 || kk > 0) ? 1u : 0u);
+        umma_commit(&pv_done[slot]);
+        if (ksplit || slot == 1) umma_commit(&empty16[d]);
+      };
+      issue_s(0, 0);
+      if (n1 > 0) issue_s(1, 0);
+      for (int k = 0; k < n0 && ok; ++k) {
+        issue_pv(0, k);
+        if (k + 1 < n0) {
+          ok = ok && mbar_wait(&pv_done[0], k & 1, p.err);  // P gives its columns back to S
+          issue_s(0, k + 1);
+        }
+        if (k < n1) {
+          issue_pv(1, k);
+          if (k + 1 < n1) {
+            ok = ok && mbar_wait(&pv_done[1], k & 1, p.err);
+            issue_s(1, k + 1);
+          }
+        }
+      }
+    }
+  } else if (warp < 8) {
+    // ---- softmax: one thread per query row
+    const int slot = warp >> 2;
+    const int r = (ksplit ? 0 : slot * 128) + (tid & 127);
+    const bool live = r < rows_cta;
+    const int grow = row0 + (live ? r : 0);
+    const int m = grow / G;
+    const int hq = h * G + grow % G;
+    const int64_t pair = static_cast<int64_t>(m) * p.Hq + hq;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + slot * 64 + lanes, tO = tmem + 128 + slot * 128 + lanes;
+    const uint32_t tQ = tmem + 384 + slot * 64 + lanes;
+    int len = 0, full = 0;
+    if (live) {
+      len = p.causal_start >= 0 ? p.causal_start + m + 1 : p.row_len[m];
+      full = p.causal_start >= 0 ? len : min(p.row_full[m], len);
+    }
+    const int lim = min(len, end), sure = min(full, end);  // keys below `sure` are visible
+    // The row of Q, scaled by a power of two so that its largest element is in [1, 2), as fp16 pairs.
+    const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + pair * kHd);
+    uint32_t ab = 0;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const uint4 w = qp[i];
+      const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ab = max(ab, __float_as_uint(to_f32(e[k])) & 0x7fffffffu);
+    }
+    const int e2 = live ? row_exponent(ab) : 0;
+    const float down = live ? __int_as_float((127 - e2) << 23) : 0.f;
+    const float fac = p.scale_log2 * __int_as_float((127 + e2) << 23);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float f[32];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 w = qp[half * 8 + i];
+        const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          f[i * 4 + k] = __uint_as_float(
+              live ? pack_half2(to_f32(e[2 * k]) * down, to_f32(e[2 * k + 1]) * down) : 0u);
+      }
+      tmem_st32(tQ + half * 32, f);
+    }
+    tc_fence_before();
+    mbar_arrive(q_full);
+
+    const int n = ksplit ? (chunks + 1 - slot) / 2 : chunks;
+    float ref = -INFINITY, sum = 0.f;
+    bool ok = true;
+    for (int k = 0; k < n && ok; ++k) {
+      const int c = ksplit ? 2 * k + slot : k;
+      const int d = c % kStages16;
+      ok = mbar_wait(&full16[d], (c / kStages16) & 1, p.err);  // the scales of the chunk
+      ok = mbar_wait(&s_full[slot], k & 1, p.err) && ok;
+      tc_fence_after();
+      float s[kChunk];
+      tmem_ld32(tS, s);
+      tmem_ld32(tS + 32, s + 32);
+      const int x0 = (c0 + c) * kChunk;
+      if (x0 + kChunk > sure) {
+        const uint64_t vis = visible64(p, m, x0, sure, lim, sh.mask_base);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j)
+          if (!((vis >> j) & 1ull)) s[j] = -INFINITY;
+      }
+      const float4* sc = sc16 + d * 8;
+      float top = -INFINITY;
+#pragma unroll
+      for (int gk = 0; gk < 8; ++gk) {
+        const float4 w = sc[gk];
+        const float* v = s + gk * 8;
+        const float mx = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+        top = fmaxf(top, fmaf(mx, fac * w.x, w.y));
+      }
+      const bool grow_ref = top > ref + kGrow;
+      if (__any_sync(0xffffffffu, grow_ref)) {
+        float a = 1.f;
+        if (grow_ref) {
+          a = ref > -INFINITY ? ex2(ref - top) : 0.f;
+          ref = top;
+          sum *= a;
+        }
+        if (k > 0) {  // O holds every P V so far: S of this chunk was issued after the last one completed
+#pragma unroll 1
+          for (int q4 = 0; q4 < 4; ++q4) {
+            float ov[32];
+            tmem_ld32(tO + q4 * 32, ov);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) ov[i] *= a;
+            tmem_st32(tO + q4 * 32, ov);
+          }
+        }
+      }
+      const float neg = ref > -INFINITY ? -ref : 0.f;
+      float pk[32];
+#pragma unroll
+      for (int gk = 0; gk < 8; ++gk) {
+        const float4 w = sc[gk];
+        const float f = fac * w.x, b = w.y + neg;
+        float acc = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+          const float p0 = ex2(fmaf(s[gk * 8 + j], f, b)), p1 = ex2(fmaf(s[gk * 8 + j + 1], f, b));
+          acc += p0 + p1;
+          pk[gk * 4 + j / 2] = __uint_as_float(pack_half2(p0, p1));
+        }
+        sum = fmaf(acc, w.z, sum);
+      }
+      tmem_st32(tS, pk);
+      tc_fence_before();
+      mbar_arrive(&p_full[slot]);
+    }
+    // ---- epilogue
+    if (n > 0) ok = mbar_wait(&pv_done[slot], (n - 1) & 1, p.err) && ok;
+    tc_fence_after();
+    const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
+    const int64_t rec = (ksplit ? 2 * blockIdx.y + slot : blockIdx.y) * pairs + pair;
+    const bool direct = p.causal_start >= 0;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (live && !direct) p.part_ml[rec] = make_float2(ref, sum);
+#pragma unroll 1
+    for (int q4 = 0; q4 < 4; ++q4) {
+      float ov[32];
+      if (n > 0) tmem_ld32(tO + q4 * 32, ov);
+      if (!live) continue;
+      if (direct) {
+        T* out = static_cast<T*>(p.out) + pair * kHd + q4 * 32;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          T v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = from_f32<T>(sum == 0.f ? 0.f : ov[i + e] * inv);
+          *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(v);
+        }
+      } else if (sum != 0.f) {
+        float* out = p.part_o + rec * kHd + q4 * 32;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<float4*>(out + i) = make_float4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+template <typename T>
+static cudaError_t launch_tc_typed(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(attn8_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  const int rows = p.M * (p.Hq / p.Hkv), tile = p.tc_ksplit ? 128 : 256;
+  return launch_k(attn8_tc_kernel<T>, dim3(p.Hkv, p.tc_splits, (rows + tile - 1) / tile), dim3(kThreads), kSmem, st,
+                  map, p);
+}
+
+cudaError_t launch_attention8_tc(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
+  return p.bf16 ? launch_tc_typed<__nv_bfloat16>(map, p, st) : launch_tc_typed<__half>(map, p, st);
+}
+
+}  // namespace atlas

@@ -8,8 +8,8 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <cmath>
 
-#include "attention.h"
 #include "kv8.h"
 
 namespace {
@@ -149,17 +149,53 @@ torch::Tensor kv8_read_pages(torch::Tensor data, torch::Tensor scale, torch::Ten
   return out;
 }
 
-// The split pass's launch shape.  Rows of a kv head (query rows times group) go in tiles of 16 while
-// they fit one tile, else of 32; the splits fill the CTA slots (two per SM for the small tile), each
-// of at least 128 keys.
-struct Shape8 {
-  int row_tile, splits;
-};
-Shape8 pick_shape8(int64_t rows, int64_t Hkv, int64_t keys, int sms) {
-  const int tile = rows <= 16 ? 16 : 32;
-  const int64_t slots = static_cast<int64_t>(sms) * (tile == 16 ? 2 : 1);
-  const int64_t ctas = Hkv * ((rows + tile - 1) / tile);
-  return {tile, static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({64, slots / ctas, (keys + 127) / 128})))};
+// The split pass's launch shape for `rows` query rows of a kv head (query rows times group).  Up to 32
+// rows go through the register tensor-core pass in tiles of 16 or 32; more through the tcgen05 pass,
+// whose CTA holds 128 rows over alternate chunks of keys or, above 128, 256 rows.  The splits fill the
+// CTA slots (two per SM for the small tile) with at least 128 keys each.
+void pick_shape8(atlas::Attn8Params& p, int64_t rows, int64_t keys, int sms) {
+  p.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 0;
+  p.tc_ksplit = rows <= 128 ? 1 : 0;
+  const int64_t tile = p.row_tile ? p.row_tile : p.tc_ksplit ? 128 : 256;
+  const int64_t slots = static_cast<int64_t>(sms) * (p.row_tile == 16 ? 2 : 1);
+  const int64_t ctas = p.Hkv * ((rows + tile - 1) / tile);
+  const int64_t most = p.row_tile == 0 && p.tc_ksplit ? 32 : 64;  // records
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>({most, slots / ctas, (keys + 127) / 128}));
+  p.tc_splits = static_cast<int>(n);
+  p.splits = static_cast<int>(most == 32 ? 2 * n : n);
+}
+
+void check_q8(torch::Tensor& q, const torch::Tensor& data, double softmax_scale) {
+  TORCH_CHECK(q.device() == data.device() && q.dim() == 3 && q.size(2) == 128 &&
+                  (q.scalar_type() == torch::kHalf || q.scalar_type() == torch::kBFloat16),
+              "q must be fp16 or bf16 [M, Hq, 128] on the cache's device");
+  TORCH_CHECK(q.size(1) >= 1 && q.size(1) % data.size(2) == 0, "Hq must be a multiple of Hkv");
+  TORCH_CHECK(q.size(0) * q.size(1) / data.size(2) <= 65535 * 128, "attention8 takes at most 65535 * 128 query rows per kv head");
+  TORCH_CHECK(softmax_scale > 0 && std::isfinite(softmax_scale), "the softmax scale must be positive and finite");
+  if (!q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
+    q = q.clone(at::MemoryFormat::Contiguous);
+}
+
+atlas::Attn8Params params8(const torch::Tensor& q, const torch::Tensor& data, const torch::Tensor& scale, int shift,
+                           const torch::Tensor& out, const torch::Tensor& prefix_pages, double softmax_scale,
+                           const torch::Tensor& err) {
+  atlas::Attn8Params p{};
+  p.q = q.data_ptr();
+  p.data = bytes(data);
+  p.scale = scale.data_ptr<float>();
+  p.out = out.data_ptr();
+  p.prefix_pages = prefix_pages.data_ptr<int>();
+  p.err = err.data_ptr<int>();
+  p.M = static_cast<int>(q.size(0));
+  p.Hq = static_cast<int>(q.size(1));
+  p.Hkv = static_cast<int>(data.size(2));
+  p.page_shift = shift;
+  p.num_pages = static_cast<int>(data.size(0));
+  p.n_prefix = static_cast<int>(prefix_pages.numel());
+  p.bf16 = q.scalar_type() == torch::kBFloat16;
+  p.scale_log2 = static_cast<float>(softmax_scale * kLog2e);
+  p.causal_start = -1;
+  return p;
 }
 
 std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data, torch::Tensor scale, c10::optional<torch::Tensor> dparams,
@@ -168,14 +204,8 @@ std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data
                          double softmax_scale, int64_t max_keys, torch::Tensor err) {
   const int shift = check_cache(data, scale, 5);
   check_err(err, data);
-  TORCH_CHECK(q.device() == data.device() && q.dim() == 3 && q.size(2) == 128 &&
-                  (q.scalar_type() == torch::kHalf || q.scalar_type() == torch::kBFloat16),
-              "q must be fp16 or bf16 [M, Hq, 128] on the cache's device");
-  if (!q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
-    q = q.clone(at::MemoryFormat::Contiguous);
+  check_q8(q, data, softmax_scale);
   const int64_t M = q.size(0), Hq = q.size(1), Hkv = data.size(2);
-  TORCH_CHECK(Hq >= 1 && Hq % Hkv == 0, "Hq must be a multiple of Hkv");
-  TORCH_CHECK(M * Hq < (int64_t{1} << 31), "attention8 size");
   check_int(prefix_pages, data, "prefix_pages");
   check_int(row_full, data, "row_full", M);
   check_int(row_len, data, "row_len", M);
@@ -193,39 +223,22 @@ std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data
   const c10::cuda::CUDAGuard guard(data.device());
   auto out = torch::empty({M, Hq * 128}, q.options());
   if (M == 0) return {out, 0};
-  atlas::Attn8Params p{};
-  p.q = q.data_ptr();
-  p.data = bytes(data);
-  p.scale = scale.data_ptr<float>();
-  p.out = out.data_ptr();
+  atlas::Attn8Params p = params8(q, data, scale, shift, out, prefix_pages, softmax_scale, err);
   p.dparams = dparams.has_value() ? dparams->data_ptr<int>() : nullptr;
   p.shared_len = static_cast<int>(shared_len);
   p.n_shared_pages = static_cast<int>(n_shared_pages);
   p.mask_base = static_cast<int>(mask_base);
-  p.prefix_pages = prefix_pages.data_ptr<int>();
   p.row_full = row_full.data_ptr<int>();
   p.row_len = row_len.data_ptr<int>();
   p.row_mask = row_mask.data_ptr<int64_t>();
   p.tail_pages = tail_pages.data_ptr<int>();
-  p.err = err.data_ptr<int>();
-  p.M = static_cast<int>(M);
-  p.Hq = static_cast<int>(Hq);
-  p.Hkv = static_cast<int>(Hkv);
-  p.page_shift = shift;
-  p.num_pages = static_cast<int>(data.size(0));
-  p.n_prefix = static_cast<int>(prefix_pages.numel());
   p.mask_words = static_cast<int>(row_mask.size(1));
   p.tail_stride = static_cast<int>(tail_pages.size(1));
-  p.bf16 = q.scalar_type() == torch::kBFloat16;
-  p.scale_log2 = static_cast<float>(softmax_scale * kLog2e);
   // A captured call is sized for the longest context its graph may see (max_keys), an eager one for its own.
   const int64_t keys = std::max<int64_t>({shared_len, n_shared_pages << shift, max_keys});
   CUtensorMap map{};
   if (keys > 0 || dparams.has_value()) {
-    const Shape8 shape =
-        pick_shape8(M * (Hq / Hkv), Hkv, keys, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
-    p.row_tile = shape.row_tile;
-    p.splits = shape.splits;
+    pick_shape8(p, M * (Hq / Hkv), keys, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
     map = map_kv8(data);
   }
   torch::Tensor parts;
@@ -238,6 +251,29 @@ std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data
   return {out, p.splits > 0 ? 2 : 1};
 }
 
+// Row m is at position start + m and sees the keys up to itself, all in prefix_pages.
+torch::Tensor attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tensor scale, torch::Tensor prefix_pages,
+                                int64_t start, double softmax_scale, torch::Tensor err) {
+  const int shift = check_cache(data, scale, 5);
+  check_err(err, data);
+  check_q8(q, data, softmax_scale);
+  check_int(prefix_pages, data, "prefix_pages");
+  const int64_t M = q.size(0), ps = data.size(3);
+  TORCH_CHECK(start >= 0 && start + M < (1 << 30), "positions must be in [0, 2^30)");
+  const int64_t n = (start + M + ps - 1) / ps;
+  TORCH_CHECK(n <= prefix_pages.numel(), start + M, " positions need ", n, " pages of ", ps,
+              " slots; the descriptor lists ", prefix_pages.numel());
+  const c10::cuda::CUDAGuard guard(data.device());
+  auto out = torch::empty({M, q.size(1) * 128}, q.options());
+  if (M == 0) return out;
+  atlas::Attn8Params p = params8(q, data, scale, shift, out, prefix_pages, softmax_scale, err);
+  p.causal_start = static_cast<int>(start);
+  p.shared_len = static_cast<int>(start + M);
+  p.tc_splits = 1;
+  check_launch(atlas::launch_attention8_tc(map_kv8(data), p, at::cuda::getCurrentCUDAStream()), "attention8_causal");
+  return out;
+}
+
 }  // namespace
 
 void register_kv8(pybind11::module& m) {
@@ -245,5 +281,6 @@ void register_kv8(pybind11::module& m) {
   m.def("kv8_copy_pages", &kv8_copy_pages, "copies of partial pages in every layer of the 8-bit cache");
   m.def("kv8_move_slots", &kv8_move_slots, "slot moves in every layer of the 8-bit cache (sources read first)");
   m.def("kv8_read_pages", &kv8_read_pages, "pages of the 8-bit cache as fp16 or bf16 values");
+  m.def("attention8_causal", &attention8_causal, "causal attention of a prefill chunk over one layer of the 8-bit cache");
   m.def("attention8", &attention8, "paged attention over one layer of the 8-bit cache");
 }

@@ -58,10 +58,15 @@ struct Attn8Params {
   int* err;
   int M, Hq, Hkv, page_shift, num_pages, n_prefix;
   int mask_words, tail_stride, splits, bf16;
-  int row_tile;  // query rows of a kv head per CTA of the split pass: 16 or 32
+  int row_tile;      // query rows of a kv head per CTA of the split pass: 16, 32, or 0 for the tcgen05 pass
+  int tc_splits;     // tcgen05 pass: key splits (grid), each two records when tc_ksplit
+  int tc_ksplit;     // both slots of a CTA hold the same 128 rows and take alternate chunks
+  int causal_start;  // >= 0: row m is at position causal_start + m and sees the keys up to itself; writes `out`
   float scale_log2;  // softmax scale * log2(e)
 };
 // map: the layer as rows of 128 bytes, box (128, min(page size, 16)), 128B swizzle.
 cudaError_t launch_attention8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st);
+
+cudaError_t launch_attention8_tc(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st);
 
 }  // namespace atlas

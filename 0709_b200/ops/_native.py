@@ -80,6 +80,7 @@ CUDA_SOURCES = [
     "bindings_kv8.cpp",
     "kv8.cu",
     "attention8.cu",
+    "attention8_tc.cu",
 ]
 
 

@@ -335,34 +335,12 @@ class CudaOps:
         return out
 
     def attention8_causal(self, q, kv_layer, desc: AttnDesc, causal_start: int, scale: float | None = None):
-        """Attention of a prefill chunk at positions ``causal_start ..`` whose own keys are in the 8-bit cache.
-
-        Compute-bound, so it runs on the tensor-core kernel of the 16-bit cache: the sequence's pages are read once
-        into a 16-bit scratch of the chunk's own (exact values, freed with the call), a cost of a few microseconds
-        per thousand keys.
-        """
-        m, hq, hd = q.shape
-        scale = 1.0 / math.sqrt(hd) if scale is None else scale
-        out = torch.empty((m, hq * hd), dtype=q.dtype, device=q.device)
-        if m == 0:
-            return out
-        ps = kv_layer.data.shape[-2]
-        total = int(causal_start) + m
-        n = (total + ps - 1) // ps
-        if causal_start < 0 or n > desc.prefix_pages.numel():
-            raise ValueError(f"{total} positions need {n} pages of {ps} slots; the descriptor lists "
-                             f"{desc.prefix_pages.numel()}")
-        pages = self._int32(desc.prefix_pages[:n])
-        limit = torch.arange(int(causal_start) + 1, total + 1, dtype=torch.int32, device=q.device)
-        listed = torch.arange(n, dtype=torch.int32, device=q.device)
-        dparams = torch.tensor([total, n, 0], dtype=torch.int32).to(q.device)
-        # The attention kernel reads its index inputs before it waits for the kernel before it, which is the read.
-        scratch = self.ext.kv8_read_pages(kv_layer.data, kv_layer.scale, pages, q.dtype == torch.bfloat16, self.err)
-        self.ext.attention(
-            q.contiguous(), scratch[None], 0, out, dparams, listed, limit, limit, desc.row_mask, desc.tail_pages,
-            self.part_o, self.part_ml, self.err, 1, True, False, True, float(scale), False,
-        )
-        counters.launches(2)
+        """Attention of a prefill chunk at positions ``causal_start ..`` whose own keys are in the 8-bit cache
+        already; the descriptor gives the page list."""
+        scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+        out = self.ext.attention8_causal(q, kv_layer.data, kv_layer.scale, desc.prefix_pages, int(causal_start), scale,
+                                         self.err)
+        counters.launches(1)
         return out
 
     def kv8_copy_pages(self, cache, copies: torch.Tensor) -> None:
