@@ -30,15 +30,24 @@ constexpr int kSmem = 1024 + kStages8 * kBytes8 + kStages16 * kBytes16 + (kStage
 constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
 }  // namespace
 
-// D (+)= A(tmem) * B(smem).
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// D (+)= A(tmem) * B(smem); B's descriptor as two words, so that the tiles of one operand differ by
+// an addition to the low word.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t desc_lo, uint32_t desc_hi,
+                                            uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+      "{\n\t.reg .pred p;\n\t.reg .b64 d;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 d, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], d, %4, {%6, %6, %6, %6}, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(0)
       : "memory");
+}
+
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 template <typename T>
@@ -187,38 +196,49 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive(&full16[d]);
     }
   } else if (warp == 13) {
-    if (lane == 0 && chunks > 0) {
-      const uint32_t idesc_s = umma_idesc_f16(128, kChunk, false, false, false);
-      const uint32_t idesc_o = umma_idesc_f16(128, kHd, false, false, true);
+    // ---- MMA issuer.  The whole warp walks the loop and one elected lane issues: addresses and
+    // descriptors then live in uniform registers.  A single thread that builds each descriptor took
+    // about 700 cycles for the eight instructions of an S tile, more than the products themselves.
+    if (chunks > 0) {
+      constexpr uint32_t idesc_s = umma_idesc_f16(128, kChunk, false, false, false);
+      constexpr uint32_t idesc_o = umma_idesc_f16(128, kHd, false, false, true);
+      constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);  // 8-row step, version, 128B swizzle
+      const uint32_t k_lo = (smem_u32(ring16) >> 4) | (16 >> 4) << 16;
+      const uint32_t v_lo = ((smem_u32(ring16) + 2 * kHalf16) >> 4) | (kHalf16 >> 4) << 16;
       const int n0 = ksplit ? (chunks + 1) / 2 : chunks, n1 = ksplit ? chunks / 2 : chunks;
+      const bool leader = elect_one();
       bool ok = mbar_wait(q_full, 0, p.err);
       tc_fence_after();
       auto issue_s = [&](int slot, int k) {
         const int c = ksplit ? 2 * k + slot : k;
         const int d = c % kStages16;
         ok = ok && mbar_wait(&full16[d], (c / kStages16) & 1, p.err);
-        if (!ok) return;
         tc_fence_after();
-        const uint32_t kb = smem_u32(ring16 + d * kBytes16);
+        const uint32_t lo = k_lo + d * (kBytes16 >> 4);
+        if (leader && ok) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_f16_ts(tmem + slot * 64, tmem + 384 + slot * 64 + kk * 8,
-                      umma_desc_sw128(kb + (kk >> 2) * kHalf16 + (kk & 3) * 32, 16, 1024), idesc_s, kk > 0);
-        umma_commit(&s_full[slot]);
+          for (int kk = 0; kk < 8; ++kk)
+            umma_f16_ts(tmem + slot * 64, tmem + 384 + slot * 64 + kk * 8,
+                        lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
+          umma_commit(&s_full[slot]);
+        }
+        __syncwarp();
       };
       auto issue_pv = [&](int slot, int k) {
         const int c = ksplit ? 2 * k + slot : k;
         const int d = c % kStages16;
         ok = ok && mbar_wait(&p_full[slot], k & 1, p.err);
-        if (!ok) return;
         tc_fence_after();
-        const uint32_t vb = smem_u32(ring16 + d * kBytes16) + 2 * kHalf16;
+        const uint32_t lo = v_lo + d * (kBytes16 >> 4);
+        if (leader && ok) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          umma_f16_ts(tmem + 128 + slot * 128, tmem + slot * 64 + kk * 8, umma_desc_sw128(vb + kk * 2048, kHalf16, 1024),
-                      idesc_o, (k > 0 || kk > 0) ? 1u : 0u);
-        umma_commit(&pv_done[slot]);
-        if (ksplit || slot == 1) umma_commit(&empty16[d]);
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16_ts(tmem + 128 + slot * 128, tmem + slot * 64 + kk * 8, lo + kk * (2048 >> 4), kDescHi, idesc_o,
+                        k > 0 || kk > 0);
+          umma_commit(&pv_done[slot]);
+          if (ksplit || slot == 1) umma_commit(&empty16[d]);
+        }
+        __syncwarp();
       };
       issue_s(0, 0);
       if (n1 > 0) issue_s(1, 0);
