@@ -7,12 +7,13 @@
 //   8-11  converters: e4m3 codes of a chunk -> fp16 operand tiles in the 128B-swizzled layout;
 //   12    TMA producer: the chunk's pages (K and V codes) and their scales;
 //   13    MMA issuer.
-// Q stays in TMEM as the A operand of S = Q K^T, P replaces S in place (fp16) and is the A operand of
-// O += P V, so the shared memory carries per 64-key chunk the codes (16 KB written, 16 KB read), the
-// fp16 tiles (32 KB written) and their reads by the MMAs (16 KB per product), and nothing for Q and P.
-// A slot's next S waits for its P V; the other slot's products run meanwhile.
+// P (fp16) is the A operand of O += P V in TMEM and so is Q of slot 0 (both slots' Q when they hold the
+// same rows) for S = Q K^T: the shared memory carries per 64-key chunk the codes (16 KB written, 16 KB
+// read), the fp16 tiles (32 KB written) and their reads by the MMAs (16 KB per product), and 32 KB of Q
+// for slot 1 when it has rows of its own, whose tile finds no room in TMEM.  S and P have columns of
+// their own, so a slot's next S is issued as soon as P is written, ahead of P V.
 //
-// TMEM columns: S/P of the slots 0-63, 64-127; O 128-255, 256-383; Q 384-447, 448-511.
+// TMEM columns: S of the slots 0-63, 64-127; O 128-255, 256-383; P 384-415, 416-447; Q 448-511.
 
 #include "attention8.cuh"
 
@@ -26,7 +27,9 @@ constexpr int kBytes8 = kChunk * kHd * 2;      // K | V codes
 constexpr int kHalf16 = kChunk * 128;          // 64 keys x 64 dimensions of fp16
 constexpr int kBytes16 = 4 * kHalf16;          // K halves | V halves
 constexpr int kThreads = 448;
-constexpr int kSmem = 1024 + kStages8 * kBytes8 + kStages16 * kBytes16 + (kStages8 + kStages16) * 128 + 256;
+constexpr int kBytesQ = 128 * kHd * 2;         // slot 1's Q: two halves of 128 rows x 128 B
+constexpr int kSmem = 1024 + kStages8 * kBytes8 + kStages16 * kBytes16 + kBytesQ + (kStages8 + kStages16) * 128 + 256;
+constexpr uint32_t kColO = 128, kColP = 384, kColQ = 448;
 constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
 }  // namespace
 
@@ -40,6 +43,18 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
       "mov.b64 d, {%2, %3};\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], d, %4, {%6, %6, %6, %6}, p;\n\t}" ::"r"(tmem_d),
       "r"(tmem_a), "r"(desc_lo), "r"(desc_hi), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(0)
+      : "memory");
+}
+
+__device__ __forceinline__ void umma_f16_ss2(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi,
+                                             uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 a, {%1, %3};\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, {%6, %6, %6, %6}, p;\n\t}" ::"r"(tmem_d),
+      "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(static_cast<uint32_t>(accumulate)), "r"(0)
       : "memory");
 }
 
@@ -57,8 +72,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring8 = smem;
   uint8_t* ring16 = ring8 + kStages8 * kBytes8;
-  // Per 8 keys of a chunk: k scale, log2(v scale), 1 / v scale (8 x float4 would waste a quarter: two arrays).
-  float4* sc8 = reinterpret_cast<float4*>(ring16 + kStages16 * kBytes16);  // [kStages8][8]
+  uint8_t* q_s = ring16 + kStages16 * kBytes16;
+  // Per 8 keys of a chunk: k scale, log2(v scale), 1 / v scale.
+  float4* sc8 = reinterpret_cast<float4*>(q_s + kBytesQ);  // [kStages8][8]
   float4* sc16 = sc8 + kStages8 * 8;                                       // [kStages16][8]
   uint64_t* full8 = reinterpret_cast<uint64_t*>(sc16 + kStages16 * 8);
   uint64_t* empty8 = full8 + kStages8;
@@ -123,34 +139,51 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int ps = 1 << p.page_shift;
 
   if (warp == 12) {
-    // ---- producer: lane g < 8 resolves 8 keys of the chunk; lane i of the first 32 loads ahead nothing else
-    bool ok = true;
+    // ---- producer.  Lane l holds page and scales of 8 keys, l & 7, of chunk l >> 3 of a window of
+    // four; the next window is loaded while this one is issued (page and scale are two dependent
+    // trips to memory: taken chunk by chunk they bound the pass at 2 TB/s).
     const int box = min(ps, 16);
-    for (int c = 0; c < chunks && ok; ++c) {
-      const int s = c % kStages8;
-      const int x = (c0 + c) * kChunk + (lane & 7) * 8;
-      int page = 0;
-      float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);
-      if (x < end) {
+    struct Window {
+      int page;
+      float4 sc;
+    };
+    auto load_window = [&](int first) {
+      Window w{0, make_float4(1.f, 0.f, 1.f, 0.f)};
+      const int c = first + (lane >> 3), x = (c0 + c) * kChunk + (lane & 7) * 8;
+      if (c < chunks && x < end) {
         const int j = x >> p.page_shift;
-        page = j < p.n_prefix ? p.prefix_pages[j] : -1;
+        const int page = j < p.n_prefix ? p.prefix_pages[j] : -1;
         if (page < 0 || page >= p.num_pages) {
           set_error(p.err, kErrBadIndex);
-          page = 0;
-        } else if (lane < 8) {
-          sc = attn8_scales(p, static_cast<int64_t>(page) * 2 * p.Hkv + h);
+        } else {
+          w.page = page;
+          w.sc = attn8_scales(p, static_cast<int64_t>(page) * 2 * p.Hkv + h);
         }
       }
-      if (c >= kStages8) ok = mbar_wait(&empty8[s], ((c / kStages8) - 1) & 1, p.err);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      return w;
+    };
+    Window cur = load_window(0), nxt = load_window(4);
+    for (int c = 0; c < chunks; ++c) {
+      if (c > 0 && (c & 3) == 0) {
+        cur = nxt;
+        nxt = load_window(c + 4);
+      }
+      const int s = c % kStages8, from = (c & 3) * 8 + (lane & 7);
+      const int page = __shfl_sync(0xffffffffu, cur.page, from);
+      float4 sc;
+      sc.x = __shfl_sync(0xffffffffu, cur.sc.x, from);
+      sc.y = __shfl_sync(0xffffffffu, cur.sc.y, from);
+      sc.z = __shfl_sync(0xffffffffu, cur.sc.z, from);
+      sc.w = 0.f;
+      bool ok = c < kStages8 || mbar_wait(&empty8[s], ((c / kStages8) - 1) & 1, p.err);
+      if (!__all_sync(0xffffffffu, ok)) break;
       if (lane < 8) sc8[s * 8 + lane] = sc;
       __syncwarp();
       if (lane == 0) mbar_arrive_expect_tx(&full8[s], kBytes8);
       __syncwarp();
-      // Lane g issues the box that starts at its 8 keys (every other lane when a box holds 16).
+      // Lane g < 8 issues the box that starts at its 8 keys (every other lane when a box holds 16).
       if (lane < 8 && (box == 8 || (lane & 1) == 0)) {
-        const int y = (page * 2 * p.Hkv + h) * ps + (x & (ps - 1));
+        const int y = (page * 2 * p.Hkv + h) * ps + (((c0 + c) * kChunk + lane * 8) & (ps - 1));
         uint8_t* dst = ring8 + s * kBytes8 + lane * 8 * kHd;
         tma_load_2d(dst, &map, &full8[s], 0, y);
         tma_load_2d(dst + kBytes8 / 2, &map, &full8[s], 0, y + p.Hkv * ps);
@@ -158,7 +191,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp >= 8 && warp < 12) {
     // ---- converters: one 16-byte piece of codes (16 dimensions of a key) per thread and step
-    const int row = (tid - 256) >> 3, piece = tid & 7;  // rows row, row + 16, ..
+    // Pieces p and p + 4 of a row would meet the same banks (its two 64-dimension halves): the upper
+    // pieces take the neighbouring row.
+    const int piece = tid & 7, upper = piece >> 2;
+    const int row = ((tid - 256) >> 3) ^ upper;  // rows row, row + 16, ..
     bool ok = true;
     for (int c = 0; c < chunks && ok; ++c) {
       const int s = c % kStages8, d = c % kStages16;
@@ -184,13 +220,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         hi.y = half_pair_hi(w[i].z);
         hi.z = half_pair_lo(w[i].w);
         hi.w = half_pair_hi(w[i].w);
-        // Pieces p and p + 4 of a row meet the same banks (the two 64-dimension halves): they store
-        // their two 16-byte parts in opposite order.
-        const int flip = piece >> 2;
-        uint8_t* half = dst + (i >> 2) * 2 * kHalf16 + flip * kHalf16;
+        uint8_t* half = dst + ((i >> 2) * 2 + upper) * kHalf16;
         const int r = row + (i & 3) * 16, at = 2 * (piece & 3);
-        *reinterpret_cast<uint4*>(half + sw128_offset(r, at + flip)) = flip ? hi : lo;
-        *reinterpret_cast<uint4*>(half + sw128_offset(r, at + (flip ^ 1))) = flip ? lo : hi;
+        *reinterpret_cast<uint4*>(half + sw128_offset(r, at)) = lo;
+        *reinterpret_cast<uint4*>(half + sw128_offset(r, at + 1)) = hi;
       }
       fence_proxy_async_smem();
       mbar_arrive(&full16[d]);
@@ -204,6 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t idesc_o = umma_idesc_f16(128, kHd, false, false, true);
       constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);  // 8-row step, version, 128B swizzle
       const uint32_t k_lo = (smem_u32(ring16) >> 4) | (16 >> 4) << 16;
+      const uint32_t q_lo = (smem_u32(q_s) >> 4) | (16 >> 4) << 16;
       const uint32_t v_lo = ((smem_u32(ring16) + 2 * kHalf16) >> 4) | (kHalf16 >> 4) << 16;
       const int n0 = ksplit ? (chunks + 1) / 2 : chunks, n1 = ksplit ? chunks / 2 : chunks;
       const bool leader = elect_one();
@@ -216,10 +250,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t lo = k_lo + d * (kBytes16 >> 4);
         if (leader && ok) {
+          if (slot == 0 || ksplit) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_f16_ts(tmem + slot * 64, tmem + 384 + slot * 64 + kk * 8,
-                        lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
+            for (int kk = 0; kk < 8; ++kk)
+              umma_f16_ts(tmem + slot * 64, tmem + kColQ + kk * 8,
+                          lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
+          } else {
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              umma_f16_ss2(tmem + 64, q_lo + (((kk >> 2) * (kBytesQ / 2) + (kk & 3) * 32) >> 4),
+                           lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
+          }
           umma_commit(&s_full[slot]);
         }
         __syncwarp();
@@ -227,13 +268,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto issue_pv = [&](int slot, int k) {
         const int c = ksplit ? 2 * k + slot : k;
         const int d = c % kStages16;
-        ok = ok && mbar_wait(&p_full[slot], k & 1, p.err);
-        tc_fence_after();
         const uint32_t lo = v_lo + d * (kBytes16 >> 4);
         if (leader && ok) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_f16_ts(tmem + 128 + slot * 128, tmem + slot * 64 + kk * 8, lo + kk * (2048 >> 4), kDescHi, idesc_o,
+            umma_f16_ts(tmem + kColO + slot * 128, tmem + kColP + slot * 32 + kk * 8, lo + kk * (2048 >> 4), kDescHi, idesc_o,
                         k > 0 || kk > 0);
           umma_commit(&pv_done[slot]);
           if (ksplit || slot == 1) umma_commit(&empty16[d]);
@@ -243,16 +282,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       issue_s(0, 0);
       if (n1 > 0) issue_s(1, 0);
       for (int k = 0; k < n0 && ok; ++k) {
-        issue_pv(0, k);
-        if (k + 1 < n0) {
-          ok = ok && mbar_wait(&pv_done[0], k & 1, p.err);  // P gives its columns back to S
-          issue_s(0, k + 1);
-        }
-        if (k < n1) {
-          issue_pv(1, k);
-          if (k + 1 < n1) {
-            ok = ok && mbar_wait(&pv_done[1], k & 1, p.err);
-            issue_s(1, k + 1);
+#pragma unroll
+        for (int slot = 0; slot < 2; ++slot) {
+          const int n = slot ? n1 : n0;
+          if (k < n) {
+            ok = ok && mbar_wait(&p_full[slot], k & 1, p.err);  // S(k) is read, P(k) written
+            tc_fence_after();
+            if (k + 1 < n) issue_s(slot, k + 1);
+            issue_pv(slot, k);
           }
         }
       }
@@ -267,8 +304,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int hq = h * G + grow % G;
     const int64_t pair = static_cast<int64_t>(m) * p.Hq + hq;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + slot * 64 + lanes, tO = tmem + 128 + slot * 128 + lanes;
-    const uint32_t tQ = tmem + 384 + slot * 64 + lanes;
+    const uint32_t tS = tmem + slot * 64 + lanes, tO = tmem + kColO + slot * 128 + lanes;
+    const uint32_t tP = tmem + kColP + slot * 32 + lanes;
     int len = 0, full = 0;
     if (live) {
       len = p.causal_start >= 0 ? p.causal_start + m + 1 : p.row_len[m];
@@ -300,8 +337,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           f[i * 4 + k] = __uint_as_float(
               live ? pack_half2(to_f32(e[2 * k]) * down, to_f32(e[2 * k + 1]) * down) : 0u);
       }
-      tmem_st32(tQ + half * 32, f);
+      if (slot == 0) {
+        tmem_st32(tmem + kColQ + half * 32 + lanes, f);
+      } else if (!ksplit) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<float4*>(q_s + half * (kBytesQ / 2) + sw128_offset(tid & 127, i)) =
+              make_float4(f[i * 4], f[i * 4 + 1], f[i * 4 + 2], f[i * 4 + 3]);
+      }
     }
+    fence_proxy_async_smem();
     tc_fence_before();
     mbar_arrive(q_full);
 
@@ -333,6 +378,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float mx = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
         top = fmaxf(top, fmaf(mx, fac * w.x, w.y));
       }
+      // P V of the chunk before: its P columns and O are free again (it was issued right behind this S).
+      if (k > 0) ok = mbar_wait(&pv_done[slot], (k - 1) & 1, p.err) && ok;
+      tc_fence_after();
       const bool grow_ref = top > ref + kGrow;
       if (__any_sync(0xffffffffu, grow_ref)) {
         float a = 1.f;
@@ -341,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ref = top;
           sum *= a;
         }
-        if (k > 0) {  // O holds every P V so far: S of this chunk was issued after the last one completed
+        if (k > 0) {
 #pragma unroll 1
           for (int q4 = 0; q4 < 4; ++q4) {
             float ov[32];
@@ -367,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         sum = fmaf(acc, w.z, sum);
       }
-      tmem_st32(tS, pk);
+      tmem_st32(tP, pk);
       tc_fence_before();
       mbar_arrive(&p_full[slot]);
     }
