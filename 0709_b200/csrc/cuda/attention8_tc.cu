@@ -7,13 +7,12 @@
 //   8-11  converters: e4m3 codes of a chunk -> fp16 operand tiles in the 128B-swizzled layout;
 //   12    TMA producer: the chunk's pages (K and V codes) and their scales;
 //   13    MMA issuer.
-// P (fp16) is the A operand of O += P V in TMEM and so is Q of slot 0 (both slots' Q when they hold the
-// same rows) for S = Q K^T: the shared memory carries per 64-key chunk the codes (16 KB written, 16 KB
-// read), the fp16 tiles (32 KB written) and their reads by the MMAs (16 KB per product), and 32 KB of Q
-// for slot 1 when it has rows of its own, whose tile finds no room in TMEM.  S and P have columns of
-// their own, so a slot's next S is issued as soon as P is written, ahead of P V.
+// S is double-buffered in TMEM, so that a slot's next scores are ready when its softmax is; P (fp16)
+// replaces its S in place and is the A operand of O += P V.  Q is read from shared memory (TMEM has no
+// room left).  Per 64-key chunk the shared memory carries the codes (16 KB written, 16 KB read), the
+// fp16 tiles (32 KB written) and per slot 16 KB of K, 32 KB of Q and 16 KB of V.
 //
-// TMEM columns: S of the slots 0-63, 64-127; O 128-255, 256-383; P 384-415, 416-447; Q 448-511.
+// TMEM columns: S/P of slot s, buffer b at 128 s + 64 b; O of slot s at 256 + 128 s.
 
 #include "attention8.cuh"
 
@@ -22,14 +21,14 @@ namespace atlas {
 namespace {
 constexpr int kChunk = 64;
 constexpr int kStages8 = 4;                    // chunks of codes in flight
-constexpr int kStages16 = 3;                   // converted chunks
 constexpr int kBytes8 = kChunk * kHd * 2;      // K | V codes
 constexpr int kHalf16 = kChunk * 128;          // 64 keys x 64 dimensions of fp16
 constexpr int kBytes16 = 4 * kHalf16;          // K halves | V halves
+constexpr int kBytesQ = 128 * kHd * 2;         // two halves of 128 rows x 128 B
+static_assert(kBytesQ == kBytes16, "slot 1's own Q takes the place of the fourth converted chunk");
 constexpr int kThreads = 448;
-constexpr int kBytesQ = 128 * kHd * 2;         // slot 1's Q: two halves of 128 rows x 128 B
-constexpr int kSmem = 1024 + kStages8 * kBytes8 + kStages16 * kBytes16 + kBytesQ + (kStages8 + kStages16) * 128 + 256;
-constexpr uint32_t kColO = 128, kColP = 384, kColQ = 448;
+constexpr int kSmem = 1024 + kStages8 * kBytes8 + 4 * kBytes16 + kBytesQ + (kStages8 + 4) * 128 + 256;
+constexpr uint32_t kColO = 256;
 constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
 }  // namespace
 
@@ -58,6 +57,31 @@ __device__ __forceinline__ void umma_f16_ss2(uint32_t tmem_d, uint32_t a_lo, uin
       : "memory");
 }
 
+// Two fp32 values as one 64-bit operand of the packed fp32 instructions.
+__device__ __forceinline__ uint64_t pair2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // One lane of a converged warp, the same one every time.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -65,23 +89,26 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
-template <typename T>
+template <typename T, bool kSplitKeys>
 __global__ void __launch_bounds__(kThreads, 1)
     attn8_tc_kernel(const __grid_constant__ CUtensorMap map, Attn8Params p) {
+  constexpr bool ksplit = kSplitKeys;
+  constexpr int kStages16 = kSplitKeys ? 4 : 3;  // converted chunks
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring8 = smem;
   uint8_t* ring16 = ring8 + kStages8 * kBytes8;
-  uint8_t* q_s = ring16 + kStages16 * kBytes16;
+  uint8_t* q_s = ring16 + 4 * kBytes16;  // slot 0 (and both slots with split keys)
+  uint8_t* q1_s = ring16 + 3 * kBytes16;
   // Per 8 keys of a chunk: k scale, log2(v scale), 1 / v scale.
   float4* sc8 = reinterpret_cast<float4*>(q_s + kBytesQ);  // [kStages8][8]
   float4* sc16 = sc8 + kStages8 * 8;                                       // [kStages16][8]
-  uint64_t* full8 = reinterpret_cast<uint64_t*>(sc16 + kStages16 * 8);
+  uint64_t* full8 = reinterpret_cast<uint64_t*>(sc16 + 4 * 8);
   uint64_t* empty8 = full8 + kStages8;
   uint64_t* full16 = empty8 + kStages8;
   uint64_t* empty16 = full16 + kStages16;
-  uint64_t* s_full = empty16 + kStages16;  // [2]
-  uint64_t* p_full = s_full + 2;           // [2], 128 arrivals
+  uint64_t* s_full = empty16 + kStages16;  // [slot][buffer]
+  uint64_t* p_full = s_full + 4;           // [2], 128 arrivals
   uint64_t* pv_done = p_full + 2;          // [2]
   uint64_t* q_full = pv_done + 2;          // 256 arrivals
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
@@ -90,7 +117,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h = blockIdx.x;
   const int G = p.Hq / p.Hkv;
   const int rows_total = p.M * G;
-  const bool ksplit = p.tc_ksplit != 0;
   // The longest causal tiles are launched first, so that the short ones fill the last wave.
   const int z = p.causal_start >= 0 ? static_cast<int>(gridDim.z - 1 - blockIdx.z) : static_cast<int>(blockIdx.z);
   const int row0 = z * (ksplit ? 128 : 256);
@@ -106,7 +132,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty16[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[s], 1);
+      mbar_init(&s_full[2 * s], 1);
+      mbar_init(&s_full[2 * s + 1], 1);
       mbar_init(&p_full[s], 128);
       mbar_init(&pv_done[s], 1);
     }
@@ -238,6 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);  // 8-row step, version, 128B swizzle
       const uint32_t k_lo = (smem_u32(ring16) >> 4) | (16 >> 4) << 16;
       const uint32_t q_lo = (smem_u32(q_s) >> 4) | (16 >> 4) << 16;
+      const uint32_t q1_lo = (smem_u32(q1_s) >> 4) | (16 >> 4) << 16;
       const uint32_t v_lo = ((smem_u32(ring16) + 2 * kHalf16) >> 4) | (kHalf16 >> 4) << 16;
       const int n0 = ksplit ? (chunks + 1) / 2 : chunks, n1 = ksplit ? chunks / 2 : chunks;
       const bool leader = elect_one();
@@ -250,18 +278,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t lo = k_lo + d * (kBytes16 >> 4);
         if (leader && ok) {
-          if (slot == 0 || ksplit) {
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              umma_f16_ts(tmem + slot * 64, tmem + kColQ + kk * 8,
-                          lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
-          } else {
-#pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              umma_f16_ss2(tmem + 64, q_lo + (((kk >> 2) * (kBytesQ / 2) + (kk & 3) * 32) >> 4),
-                           lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
-          }
-          umma_commit(&s_full[slot]);
+          for (int kk = 0; kk < 8; ++kk)
+            umma_f16_ss2(tmem + slot * 128 + (k & 1) * 64,
+                         (ksplit || slot == 0 ? q_lo : q1_lo) + (((kk >> 2) * (kBytesQ / 2) + (kk & 3) * 32) >> 4),
+                         lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
+          umma_commit(&s_full[slot * 2 + (k & 1)]);
         }
         __syncwarp();
       };
@@ -272,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (leader && ok) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_f16_ts(tmem + kColO + slot * 128, tmem + kColP + slot * 32 + kk * 8, lo + kk * (2048 >> 4), kDescHi, idesc_o,
+            umma_f16_ts(tmem + kColO + slot * 128, tmem + slot * 128 + (k & 1) * 64 + kk * 8, lo + kk * (2048 >> 4), kDescHi, idesc_o,
                         k > 0 || kk > 0);
           umma_commit(&pv_done[slot]);
           if (ksplit || slot == 1) umma_commit(&empty16[d]);
@@ -286,9 +308,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int slot = 0; slot < 2; ++slot) {
           const int n = slot ? n1 : n0;
           if (k < n) {
-            ok = ok && mbar_wait(&p_full[slot], k & 1, p.err);  // S(k) is read, P(k) written
+            if (k + 1 < n) {  // its buffer holds P(k - 1) until that P V is done
+              ok = ok && (k == 0 || mbar_wait(&pv_done[slot], (k - 1) & 1, p.err));
+              issue_s(slot, k + 1);
+            }
+            ok = ok && mbar_wait(&p_full[slot], k & 1, p.err);
             tc_fence_after();
-            if (k + 1 < n) issue_s(slot, k + 1);
             issue_pv(slot, k);
           }
         }
@@ -304,8 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int hq = h * G + grow % G;
     const int64_t pair = static_cast<int64_t>(m) * p.Hq + hq;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + slot * 64 + lanes, tO = tmem + kColO + slot * 128 + lanes;
-    const uint32_t tP = tmem + kColP + slot * 32 + lanes;
+    const uint32_t tS0 = tmem + slot * 128 + lanes, tO = tmem + kColO + slot * 128 + lanes;
     int len = 0, full = 0;
     if (live) {
       len = p.causal_start >= 0 ? p.causal_start + m + 1 : p.row_len[m];
@@ -337,17 +361,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           f[i * 4 + k] = __uint_as_float(
               live ? pack_half2(to_f32(e[2 * k]) * down, to_f32(e[2 * k + 1]) * down) : 0u);
       }
-      if (slot == 0) {
-        tmem_st32(tmem + kColQ + half * 32 + lanes, f);
-      } else if (!ksplit) {
+      if (slot == 0 || !ksplit) {
+        uint8_t* q = slot == 0 ? q_s : q1_s;
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float4*>(q_s + half * (kBytesQ / 2) + sw128_offset(tid & 127, i)) =
+          *reinterpret_cast<float4*>(q + half * (kBytesQ / 2) + sw128_offset(tid & 127, i)) =
               make_float4(f[i * 4], f[i * 4 + 1], f[i * 4 + 2], f[i * 4 + 3]);
       }
     }
     fence_proxy_async_smem();
-    tc_fence_before();
     mbar_arrive(q_full);
 
     const int n = ksplit ? (chunks + 1 - slot) / 2 : chunks;
@@ -357,8 +379,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int c = ksplit ? 2 * k + slot : k;
       const int d = c % kStages16;
       ok = mbar_wait(&full16[d], (c / kStages16) & 1, p.err);  // the scales of the chunk
-      ok = mbar_wait(&s_full[slot], k & 1, p.err) && ok;
+      ok = mbar_wait(&s_full[slot * 2 + (k & 1)], (k >> 1) & 1, p.err) && ok;
       tc_fence_after();
+      const uint32_t tS = tS0 + (k & 1) * 64;
       float s[kChunk];
       tmem_ld32(tS, s);
       tmem_ld32(tS + 32, s + 32);
@@ -375,12 +398,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int gk = 0; gk < 8; ++gk) {
         const float4 w = sc[gk];
         const float* v = s + gk * 8;
-        const float mx = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+        const float mx = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
         top = fmaxf(top, fmaf(mx, fac * w.x, w.y));
       }
-      // P V of the chunk before: its P columns and O are free again (it was issued right behind this S).
-      if (k > 0) ok = mbar_wait(&pv_done[slot], (k - 1) & 1, p.err) && ok;
-      tc_fence_after();
       const bool grow_ref = top > ref + kGrow;
       if (__any_sync(0xffffffffu, grow_ref)) {
         float a = 1.f;
@@ -389,7 +409,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           ref = top;
           sum *= a;
         }
-        if (k > 0) {
+        if (k > 0) {  // O has to hold P V of every chunk before
+          ok = mbar_wait(&pv_done[slot], (k - 1) & 1, p.err) && ok;
+          tc_fence_after();
 #pragma unroll 1
           for (int q4 = 0; q4 < 4; ++q4) {
             float ov[32];
@@ -405,17 +427,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int gk = 0; gk < 8; ++gk) {
         const float4 w = sc[gk];
-        const float f = fac * w.x, b = w.y + neg;
-        float acc = 0.f;
+        const uint64_t f = pair2(fac * w.x, fac * w.x), b = pair2(w.y + neg, w.y + neg);
+        uint64_t acc = 0;
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
-          const float p0 = ex2(fmaf(s[gk * 8 + j], f, b)), p1 = ex2(fmaf(s[gk * 8 + j + 1], f, b));
-          acc += p0 + p1;
+          float p0, p1;
+          unpair2(fma2(pair2(s[gk * 8 + j], s[gk * 8 + j + 1]), f, b), p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          acc = add2(acc, pair2(p0, p1));
           pk[gk * 4 + j / 2] = __uint_as_float(pack_half2(p0, p1));
         }
-        sum = fmaf(acc, w.z, sum);
+        float a0, a1;
+        unpair2(acc, a0, a1);
+        sum = fmaf(a0 + a1, w.z, sum);
       }
-      tmem_st32(tP, pk);
+      tmem_st32(tS, pk);
       tc_fence_before();
       mbar_arrive(&p_full[slot]);
     }
@@ -454,17 +481,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-template <typename T>
+template <typename T, bool kSplitKeys>
 static cudaError_t launch_tc_typed(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(attn8_tc_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  const cudaError_t e =
+      cudaFuncSetAttribute(attn8_tc_kernel<T, kSplitKeys>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  const int rows = p.M * (p.Hq / p.Hkv), tile = p.tc_ksplit ? 128 : 256;
-  return launch_k(attn8_tc_kernel<T>, dim3(p.Hkv, p.tc_splits, (rows + tile - 1) / tile), dim3(kThreads), kSmem, st,
-                  map, p);
+  const int rows = p.M * (p.Hq / p.Hkv), tile = kSplitKeys ? 128 : 256;
+  return launch_k(attn8_tc_kernel<T, kSplitKeys>, dim3(p.Hkv, p.tc_splits, (rows + tile - 1) / tile), dim3(kThreads),
+                  kSmem, st, map, p);
 }
 
 cudaError_t launch_attention8_tc(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
-  return p.bf16 ? launch_tc_typed<__nv_bfloat16>(map, p, st) : launch_tc_typed<__half>(map, p, st);
+  if (p.tc_ksplit)
+    return p.bf16 ? launch_tc_typed<__nv_bfloat16, true>(map, p, st) : launch_tc_typed<__half, true>(map, p, st);
+  return p.bf16 ? launch_tc_typed<__nv_bfloat16, false>(map, p, st) : launch_tc_typed<__half, false>(map, p, st);
 }
 
 }  // namespace atlas
