@@ -2,11 +2,12 @@
 //
 // One CTA holds two tiles ("slots") of 128 query rows of one kv head: two different row tiles over
 // the same keys, or -- when one tile holds all rows -- the same rows over alternate 64-key chunks,
-// each slot then being a split of its own.  14 warps:
+// each slot then being a split of its own.  15 warps:
 //   0-7   softmax, one thread per query row (0-3 slot 0, 4-7 slot 1);
 //   8-11  converters: e4m3 codes of a chunk -> fp16 operand tiles in the 128B-swizzled layout;
 //   12    TMA producer: the chunk's pages (K and V codes) and their scales;
-//   13    MMA issuer.
+//   13-14 MMA issuers, one per slot (one for both spent its time in turn on waits and issue: 2450
+//         cycles per pair of S and P V tiles whose products take 1280).
 // S is double-buffered in TMEM, so that a slot's next scores are ready when its softmax is; P (fp16)
 // replaces its S in place and is the A operand of O += P V.  Q is read from shared memory (TMEM has no
 // room left).  Per 64-key chunk the shared memory carries the codes (16 KB written, 16 KB read), the
@@ -26,7 +27,7 @@ constexpr int kHalf16 = kChunk * 128;          // 64 keys x 64 dimensions of fp1
 constexpr int kBytes16 = 4 * kHalf16;          // K halves | V halves
 constexpr int kBytesQ = 128 * kHd * 2;         // two halves of 128 rows x 128 B
 static_assert(kBytesQ == kBytes16, "slot 1's own Q takes the place of the fourth converted chunk");
-constexpr int kThreads = 448;
+constexpr int kThreads = 480;
 constexpr int kSmem = 1024 + kStages8 * kBytes8 + 4 * kBytes16 + kBytesQ + (kStages8 + 4) * 128 + 256;
 constexpr uint32_t kColO = 256;
 constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < kStages16; ++s) {
       mbar_init(&full16[s], 128);
-      mbar_init(&empty16[s], 1);
+      mbar_init(&empty16[s], ksplit ? 1 : 2);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[2 * s], 1);
@@ -255,67 +256,51 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();
       mbar_arrive(&full16[d]);
     }
-  } else if (warp == 13) {
-    // ---- MMA issuer.  The whole warp walks the loop and one elected lane issues: addresses and
-    // descriptors then live in uniform registers.  A single thread that builds each descriptor took
-    // about 700 cycles for the eight instructions of an S tile, more than the products themselves.
-    if (chunks > 0) {
+  } else if (warp >= 13) {
+    // ---- MMA issuer of a slot.  The whole warp walks the loop and one elected lane issues: addresses
+    // and descriptors then live in uniform registers (a single thread that builds each descriptor took
+    // about 700 cycles for the eight instructions of an S tile, more than the products themselves).
+    const int slot = warp - 13;
+    const int n = ksplit ? (chunks + 1 - slot) / 2 : chunks;
+    if (n > 0) {
       constexpr uint32_t idesc_s = umma_idesc_f16(128, kChunk, false, false, false);
       constexpr uint32_t idesc_o = umma_idesc_f16(128, kHd, false, false, true);
       constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);  // 8-row step, version, 128B swizzle
+      const uint32_t q_lo = (smem_u32(ksplit || slot == 0 ? q_s : q1_s) >> 4) | (16 >> 4) << 16;
       const uint32_t k_lo = (smem_u32(ring16) >> 4) | (16 >> 4) << 16;
-      const uint32_t q_lo = (smem_u32(q_s) >> 4) | (16 >> 4) << 16;
-      const uint32_t q1_lo = (smem_u32(q1_s) >> 4) | (16 >> 4) << 16;
       const uint32_t v_lo = ((smem_u32(ring16) + 2 * kHalf16) >> 4) | (kHalf16 >> 4) << 16;
-      const int n0 = ksplit ? (chunks + 1) / 2 : chunks, n1 = ksplit ? chunks / 2 : chunks;
+      const uint32_t tS0 = tmem + slot * 128, tO = tmem + kColO + slot * 128;
       const bool leader = elect_one();
       bool ok = mbar_wait(q_full, 0, p.err);
-      tc_fence_after();
-      auto issue_s = [&](int slot, int k) {
-        const int c = ksplit ? 2 * k + slot : k;
-        const int d = c % kStages16;
-        ok = ok && mbar_wait(&full16[d], (c / kStages16) & 1, p.err);
-        tc_fence_after();
-        const uint32_t lo = k_lo + d * (kBytes16 >> 4);
-        if (leader && ok) {
+      for (int k = 0; k <= n && ok; ++k) {
+        if (k < n) {  // S(k); its buffer holds P(k - 2) until that P V is done
+          const int c = ksplit ? 2 * k + slot : k, d = c % kStages16;
+          if (k >= 2) ok = mbar_wait(&pv_done[slot], k & 1, p.err);
+          ok = ok && mbar_wait(&full16[d], (c / kStages16) & 1, p.err);
+          tc_fence_after();
+          const uint32_t lo = k_lo + d * (kBytes16 >> 4);
+          if (leader && ok) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_f16_ss2(tmem + slot * 128 + (k & 1) * 64,
-                         (ksplit || slot == 0 ? q_lo : q1_lo) + (((kk >> 2) * (kBytesQ / 2) + (kk & 3) * 32) >> 4),
-                         lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
-          umma_commit(&s_full[slot * 2 + (k & 1)]);
-        }
-        __syncwarp();
-      };
-      auto issue_pv = [&](int slot, int k) {
-        const int c = ksplit ? 2 * k + slot : k;
-        const int d = c % kStages16;
-        const uint32_t lo = v_lo + d * (kBytes16 >> 4);
-        if (leader && ok) {
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_f16_ts(tmem + kColO + slot * 128, tmem + slot * 128 + (k & 1) * 64 + kk * 8, lo + kk * (2048 >> 4), kDescHi, idesc_o,
-                        k > 0 || kk > 0);
-          umma_commit(&pv_done[slot]);
-          if (ksplit || slot == 1) umma_commit(&empty16[d]);
-        }
-        __syncwarp();
-      };
-      issue_s(0, 0);
-      if (n1 > 0) issue_s(1, 0);
-      for (int k = 0; k < n0 && ok; ++k) {
-#pragma unroll
-        for (int slot = 0; slot < 2; ++slot) {
-          const int n = slot ? n1 : n0;
-          if (k < n) {
-            if (k + 1 < n) {  // its buffer holds P(k - 1) until that P V is done
-              ok = ok && (k == 0 || mbar_wait(&pv_done[slot], (k - 1) & 1, p.err));
-              issue_s(slot, k + 1);
-            }
-            ok = ok && mbar_wait(&p_full[slot], k & 1, p.err);
-            tc_fence_after();
-            issue_pv(slot, k);
+            for (int kk = 0; kk < 8; ++kk)
+              umma_f16_ss2(tS0 + (k & 1) * 64, q_lo + (((kk >> 2) * (kBytesQ / 2) + (kk & 3) * 32) >> 4),
+                           lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
+            umma_commit(&s_full[slot * 2 + (k & 1)]);
           }
+          __syncwarp();
+        }
+        if (k > 0) {  // P(k - 1) V
+          const int j = k - 1, c = ksplit ? 2 * j + slot : j, d = c % kStages16;
+          ok = ok && mbar_wait(&p_full[slot], j & 1, p.err);
+          tc_fence_after();
+          const uint32_t lo = v_lo + d * (kBytes16 >> 4);
+          if (leader && ok) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16_ts(tO, tS0 + (j & 1) * 64 + kk * 8, lo + kk * (2048 >> 4), kDescHi, idesc_o, j > 0 || kk > 0);
+            umma_commit(&pv_done[slot]);
+            umma_commit(&empty16[d]);
+          }
+          __syncwarp();
         }
       }
     }
