@@ -2,11 +2,12 @@
 //
 // One CTA holds two tiles ("slots") of 128 query rows of one kv head: two different row tiles over
 // the same keys, or -- when one tile holds all rows -- the same rows over alternate 64-key chunks,
-// each slot then being a split of its own.  15 warps:
+// each slot then being a split of its own.  19 warps:
 //   0-7   softmax, one thread per query row (0-3 slot 0, 4-7 slot 1);
-//   8-11  converters: e4m3 codes of a chunk -> fp16 operand tiles in the 128B-swizzled layout;
-//   12    TMA producer: the chunk's pages (K and V codes) and their scales;
-//   13-14 MMA issuers, one per slot (one for both spent its time in turn on waits and issue: 2450
+//   8-15  converters: e4m3 codes of a chunk -> fp16 operand tiles in the 128B-swizzled layout (two
+//         groups of four warps, alternate chunks);
+//   16    TMA producer: the chunk's pages (K and V codes) and their scales;
+//   17-18 MMA issuers, one per slot (one for both spent its time in turn on waits and issue: 2450
 //         cycles per pair of S and P V tiles whose products take 1280).
 // S is double-buffered in TMEM, so that a slot's next scores are ready when its softmax is; P (fp16)
 // replaces its S in place and is the A operand of O += P V.  Q is read from shared memory (TMEM has no
@@ -27,7 +28,7 @@ constexpr int kHalf16 = kChunk * 128;          // 64 keys x 64 dimensions of fp1
 constexpr int kBytes16 = 4 * kHalf16;          // K halves | V halves
 constexpr int kBytesQ = 128 * kHd * 2;         // two halves of 128 rows x 128 B
 static_assert(kBytesQ == kBytes16, "slot 1's own Q takes the place of the fourth converted chunk");
-constexpr int kThreads = 480;
+constexpr int kThreads = 608;
 constexpr int kSmem = 1024 + kStages8 * kBytes8 + 4 * kBytes16 + kBytesQ + (kStages8 + 4) * 128 + 256;
 constexpr uint32_t kColO = 256;
 constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
@@ -83,6 +84,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Keys whose bit is 0 get no weight.
+__device__ __forceinline__ void hide(float* s, uint64_t vis) {
+  const uint32_t v = static_cast<uint32_t>(vis);
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (!((v >> j) & 1u)) s[j] = -INFINITY;
+}
+
+// Store 16 consecutive 32-bit columns of this thread's TMEM lane (warp-collective).
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
 // One lane of a converged warp, the same one every time.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -133,8 +153,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&empty16[s], ksplit ? 1 : 2);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&s_full[2 * s], 1);
-      mbar_init(&s_full[2 * s + 1], 1);
+      mbar_init(&s_full[2 * s], 2);
+      mbar_init(&s_full[2 * s + 1], 2);
       mbar_init(&p_full[s], 128);
       mbar_init(&pv_done[s], 1);
     }
@@ -166,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int chunks = max(0, min(chunks_all, c0 + per) - c0);
   const int ps = 1 << p.page_shift;
 
-  if (warp == 12) {
+  if (warp == 16) {
     // ---- producer.  Lane l holds page and scales of 8 keys, l & 7, of chunk l >> 3 of a window of
     // four; the next window is loaded while this one is issued (page and scale are two dependent
     // trips to memory: taken chunk by chunk they bound the pass at 2 TB/s).
@@ -217,19 +237,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_2d(dst + kBytes8 / 2, &map, &full8[s], 0, y + p.Hkv * ps);
       }
     }
-  } else if (warp >= 8 && warp < 12) {
+  } else if (warp >= 8 && warp < 16) {
     // ---- converters: one 16-byte piece of codes (16 dimensions of a key) per thread and step
     // Pieces p and p + 4 of a row would meet the same banks (its two 64-dimension halves): the upper
     // pieces take the neighbouring row.
     const int piece = tid & 7, upper = piece >> 2;
-    const int row = ((tid - 256) >> 3) ^ upper;  // rows row, row + 16, ..
+    const int row = ((tid & 127) >> 3) ^ upper;  // rows row, row + 16, ..
     bool ok = true;
-    for (int c = 0; c < chunks && ok; ++c) {
+    for (int c = (warp - 8) >> 2; c < chunks && ok; c += 2) {
       const int s = c % kStages8, d = c % kStages16;
       ok = mbar_wait(&full8[s], (c / kStages8) & 1, p.err);
       if (ok && c >= kStages16) ok = mbar_wait(&empty16[d], ((c / kStages16) - 1) & 1, p.err);
       if (!ok) break;
-      if (tid - 256 < 8) sc16[d * 8 + tid - 256] = sc8[s * 8 + tid - 256];
+      if ((tid & 127) < 8) sc16[d * 8 + (tid & 127)] = sc8[s * 8 + (tid & 127)];
       const uint8_t* src = ring8 + s * kBytes8;
       uint8_t* dst = ring16 + d * kBytes16;
       uint4 w[8];
@@ -256,11 +276,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();
       mbar_arrive(&full16[d]);
     }
-  } else if (warp >= 13) {
+  } else if (warp >= 17) {
     // ---- MMA issuer of a slot.  The whole warp walks the loop and one elected lane issues: addresses
     // and descriptors then live in uniform registers (a single thread that builds each descriptor took
     // about 700 cycles for the eight instructions of an S tile, more than the products themselves).
-    const int slot = warp - 13;
+    const int slot = warp - 17;
     const int n = ksplit ? (chunks + 1 - slot) / 2 : chunks;
     if (n > 0) {
       constexpr uint32_t idesc_s = umma_idesc_f16(128, kChunk, false, false, false);
@@ -285,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               umma_f16_ss2(tS0 + (k & 1) * 64, q_lo + (((kk >> 2) * (kBytesQ / 2) + (kk & 3) * 32) >> 4),
                            lo + (((kk >> 2) * kHalf16 + (kk & 3) * 32) >> 4), kDescHi, idesc_s, kk > 0);
             umma_commit(&s_full[slot * 2 + (k & 1)]);
+            mbar_arrive(&s_full[slot * 2 + (k & 1)]);  // passes on what full16 covers: the chunk's scales
           }
           __syncwarp();
         }
@@ -363,28 +384,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int k = 0; k < n && ok; ++k) {
       const int c = ksplit ? 2 * k + slot : k;
       const int d = c % kStages16;
-      ok = mbar_wait(&full16[d], (c / kStages16) & 1, p.err);  // the scales of the chunk
-      ok = mbar_wait(&s_full[slot * 2 + (k & 1)], (k >> 1) & 1, p.err) && ok;
+      ok = mbar_wait(&s_full[slot * 2 + (k & 1)], (k >> 1) & 1, p.err);
       tc_fence_after();
       const uint32_t tS = tS0 + (k & 1) * 64;
-      float s[kChunk];
-      tmem_ld32(tS, s);
-      tmem_ld32(tS + 32, s + 32);
       const int x0 = (c0 + c) * kChunk;
-      if (x0 + kChunk > sure) {
-        const uint64_t vis = visible64(p, m, x0, sure, lim, sh.mask_base);
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j)
-          if (!((vis >> j) & 1ull)) s[j] = -INFINITY;
-      }
+      const bool partial = x0 + kChunk > sure;
+      const uint64_t vis = partial ? visible64(p, m, x0, sure, lim, sh.mask_base) : ~0ull;
       const float4* sc = sc16 + d * 8;
+      // Two passes over S, 32 keys at a time (a whole row of S would not fit the registers that 19
+      // warps leave): the maximum, then the weights.
       float top = -INFINITY;
 #pragma unroll
-      for (int gk = 0; gk < 8; ++gk) {
-        const float4 w = sc[gk];
-        const float* v = s + gk * 8;
-        const float mx = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
-        top = fmaxf(top, fmaf(mx, fac * w.x, w.y));
+      for (int half = 0; half < 2; ++half) {
+        float s[32];
+        tmem_ld32(tS + half * 32, s);
+        if (partial) hide(s, vis >> (half * 32));
+#pragma unroll
+        for (int gk = 0; gk < 4; ++gk) {
+          const float4 w = sc[half * 4 + gk];
+          const float* v = s + gk * 8;
+          const float mx = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
+          top = fmaxf(top, fmaf(mx, fac * w.x, w.y));
+        }
       }
       const bool grow_ref = top > ref + kGrow;
       if (__any_sync(0xffffffffu, grow_ref)) {
@@ -408,26 +429,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float neg = ref > -INFINITY ? -ref : 0.f;
-      float pk[32];
 #pragma unroll
-      for (int gk = 0; gk < 8; ++gk) {
-        const float4 w = sc[gk];
-        const uint64_t f = pair2(fac * w.x, fac * w.x), b = pair2(w.y + neg, w.y + neg);
-        uint64_t acc = 0;
+      for (int half = 0; half < 2; ++half) {
+        float s[32], pk[16];
+        tmem_ld32(tS + half * 32, s);
+        if (partial) hide(s, vis >> (half * 32));
 #pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          float p0, p1;
-          unpair2(fma2(pair2(s[gk * 8 + j], s[gk * 8 + j + 1]), f, b), p0, p1);
-          p0 = ex2(p0);
-          p1 = ex2(p1);
-          acc = add2(acc, pair2(p0, p1));
-          pk[gk * 4 + j / 2] = __uint_as_float(pack_half2(p0, p1));
+        for (int gk = 0; gk < 4; ++gk) {
+          const float4 w = sc[half * 4 + gk];
+          const uint64_t f = pair2(fac * w.x, fac * w.x), b = pair2(w.y + neg, w.y + neg);
+          uint64_t acc = 0;
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            float p0, p1;
+            unpair2(fma2(pair2(s[gk * 8 + j], s[gk * 8 + j + 1]), f, b), p0, p1);
+            p0 = ex2(p0);
+            p1 = ex2(p1);
+            acc = add2(acc, pair2(p0, p1));
+            pk[gk * 4 + j / 2] = __uint_as_float(pack_half2(p0, p1));
+          }
+          float a0, a1;
+          unpair2(acc, a0, a1);
+          sum = fmaf(a0 + a1, w.z, sum);
         }
-        float a0, a1;
-        unpair2(acc, a0, a1);
-        sum = fmaf(a0 + a1, w.z, sum);
+        tmem_st16(tS + half * 16, pk);  // over keys of the first half, which are read
       }
-      tmem_st32(tS, pk);
       tc_fence_before();
       mbar_arrive(&p_full[slot]);
     }
