@@ -459,10 +459,13 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
   }
 }
 
-// One warp per (row, q head): the row's private tail keys, then the splits' records in split order
-// (a fixed order: the result does not depend on timing).
+// One warp per (row, q head): the splits' records, joined in split order, and the row's private tail
+// keys (a fixed order: the result does not depend on timing).  Bound by latency: the records are read
+// in one trip and the partial rows in batches of 16 (one record after the other took 24 us for 37
+// splits), while the tail's keys are on their way.
 template <typename T>
 __global__ void __launch_bounds__(128) attn8_merge_kernel(Attn8Params p) {
+  constexpr int kBatch = 16;
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -470,6 +473,17 @@ __global__ void __launch_bounds__(128) attn8_merge_kernel(Attn8Params p) {
   const int64_t pair = static_cast<int64_t>(blockIdx.x) * 4 + warp;
   if (pair >= pairs) return;
   const int m = static_cast<int>(pair / p.Hq), hq = static_cast<int>(pair % p.Hq);
+  const int S = p.splits;
+  // Lane i holds records i and i + 32 (at most 64).
+  float2 ml0 = make_float2(-INFINITY, 0.f), ml1 = ml0;
+  if (lane < S) ml0 = __ldcg(p.part_ml + lane * pairs + pair);
+  if (lane + 32 < S) ml1 = __ldcg(p.part_ml + (lane + 32) * pairs + pair);
+  const float* po = p.part_o + pair * kHd + lane * 4;
+  float4 ov[kBatch];
+#pragma unroll
+  for (int j = 0; j < kBatch; ++j)
+    if (j < S) ov[j] = __ldcg(reinterpret_cast<const float4*>(po + j * pairs * kHd));
+
   const Attn8Shape s = attn8_shape(p);
   const int len = p.row_len[m], full = min(p.row_full[m], len);
   float o[4] = {0.f, 0.f, 0.f, 0.f}, ref = -INFINITY, l = 0.f;
@@ -478,19 +492,35 @@ __global__ void __launch_bounds__(128) attn8_merge_kernel(Attn8Params p) {
     load_q4<T>(p, pair, lane, q);
     fold_keys8<true>(p, s, m, hq / (p.Hq / p.Hkv), lane, q, s.shared_end, len, full, len, ref, l, o);
   }
-  for (int i = 0; i < p.splits; ++i) {
-    const int64_t rec = i * pairs + pair;
-    const float2 ml = __ldcg(p.part_ml + rec);
-    if (ml.y == 0.f) continue;  // no key of this row in the split (a NaN sum goes on)
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + rec * kHd + lane * 4));
-    const float nm = fmaxf(ref, ml.x);
-    const float a = ref > -INFINITY ? exp2f(ref - nm) : 0.f, b = exp2f(ml.x - nm);
-    o[0] = o[0] * a + v.x * b;
-    o[1] = o[1] * a + v.y * b;
-    o[2] = o[2] * a + v.z * b;
-    o[3] = o[3] * a + v.w * b;
-    l = l * a + ml.y * b;
-    ref = nm;
+
+  // A record without keys has sum 0 and no partial row; a NaN sum keeps its weight, so that it shows.
+  const bool has0 = ml0.y != 0.f, has1 = ml1.y != 0.f;
+  const float top = warp_max(fmaxf(has0 ? ml0.x : -INFINITY, has1 ? ml1.x : -INFINITY));
+  const float mx = fmaxf(top, ref);
+  const float w0 = !has0 ? 0.f : mx > -INFINITY ? ex2(ml0.x - mx) : 1.f;
+  const float w1 = !has1 ? 0.f : mx > -INFINITY ? ex2(ml1.x - mx) : 1.f;
+  const float own = ref > -INFINITY ? ex2(ref - mx) : (l != 0.f ? 1.f : 0.f);
+  l = l * own + warp_sum((has0 ? w0 * ml0.y : 0.f) + (has1 ? w1 * ml1.y : 0.f));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= own;
+  const uint32_t some0 = __ballot_sync(0xffffffffu, has0), some1 = __ballot_sync(0xffffffffu, has1);
+  for (int s0 = 0; s0 < S; s0 += kBatch) {
+    if (s0 > 0) {
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (s0 + j < S) ov[j] = __ldcg(reinterpret_cast<const float4*>(po + (s0 + j) * pairs * kHd));
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int i = s0 + j;
+      const float w = __shfl_sync(0xffffffffu, i < 32 ? w0 : w1, i & 31);
+      if (i < S && (((i < 32 ? some0 : some1) >> (i & 31)) & 1u)) {  // warp-uniform
+        o[0] = fmaf(w, ov[j].x, o[0]);
+        o[1] = fmaf(w, ov[j].y, o[1]);
+        o[2] = fmaf(w, ov[j].z, o[2]);
+        o[3] = fmaf(w, ov[j].w, o[3]);
+      }
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;  // a row without a key answers zero
   T v[4];

@@ -342,39 +342,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       full = p.causal_start >= 0 ? len : min(p.row_full[m], len);
     }
     const int lim = min(len, end), sure = min(full, end);  // keys below `sure` are visible
-    // The row of Q, scaled by a power of two so that its largest element is in [1, 2), as fp16 pairs.
-    const uint4* qp = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + pair * kHd);
-    uint32_t ab = 0;
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
-      const uint4 w = qp[i];
-      const T* e = reinterpret_cast<const T*>(&w);
+    // The warp's 32 rows of Q, each scaled by a power of two so that its largest element is in [1, 2),
+    // as fp16 in the swizzled layout.  A row is read by the whole warp (a thread per row touches 32
+    // lines with every load: 16,000 cycles for the CTA's rows), lane i keeps row i's factor.
+    int e2 = 0;
+    {
+      uint8_t* qs = slot == 0 ? q_s : q1_s;
+      const int first = (ksplit ? 0 : slot * 128) + (warp & 3) * 32;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32; i0 += 16) {
+        uint2 w[16];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ab = max(ab, __float_as_uint(to_f32(e[k])) & 0x7fffffffu);
+        for (int i = 0; i < 16; ++i) {
+          const int rr = row0 + first + i0 + i;
+          w[i] = make_uint2(0, 0);
+          if (first + i0 + i < rows_cta)
+            w[i] = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) +
+                                                   (static_cast<int64_t>(rr / G) * p.Hq + h * G + rr % G) * kHd + lane * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const T* e = reinterpret_cast<const T*>(&w[i]);
+          const float q[4] = {to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
+          uint32_t ab = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) ab = max(ab, __float_as_uint(q[k]) & 0x7fffffffu);
+          const int x2 = row_exponent(__reduce_max_sync(0xffffffffu, ab));
+          const float down = __int_as_float((127 - x2) << 23);
+          if (lane == i0 + i) e2 = x2;
+          if (slot == 0 || !ksplit) {
+            const int row = (warp & 3) * 32 + i0 + i;
+            *reinterpret_cast<uint2*>(qs + (lane >> 4) * (kBytesQ / 2) + sw128_offset(row, (lane & 15) >> 1) +
+                                      (lane & 1) * 8) =
+                make_uint2(pack_half2(q[0] * down, q[1] * down), pack_half2(q[2] * down, q[3] * down));
+          }
+        }
+      }
     }
-    const int e2 = live ? row_exponent(ab) : 0;
-    const float down = live ? __int_as_float((127 - e2) << 23) : 0.f;
     const float fac = p.scale_log2 * __int_as_float((127 + e2) << 23);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float f[32];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 w = qp[half * 8 + i];
-        const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          f[i * 4 + k] = __uint_as_float(
-              live ? pack_half2(to_f32(e[2 * k]) * down, to_f32(e[2 * k + 1]) * down) : 0u);
-      }
-      if (slot == 0 || !ksplit) {
-        uint8_t* q = slot == 0 ? q_s : q1_s;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<float4*>(q + half * (kBytesQ / 2) + sw128_offset(tid & 127, i)) =
-              make_float4(f[i * 4], f[i * 4 + 1], f[i * 4 + 2], f[i * 4 + 3]);
-      }
-    }
     fence_proxy_async_smem();
     mbar_arrive(q_full);
 
@@ -461,29 +466,39 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (n > 0) ok = mbar_wait(&pv_done[slot], (n - 1) & 1, p.err) && ok;
     tc_fence_after();
     const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
-    const int64_t rec = (ksplit ? 2 * blockIdx.y + slot : blockIdx.y) * pairs + pair;
+    const int64_t record = (ksplit ? 2 * blockIdx.y + slot : blockIdx.y) * pairs;
     const bool direct = p.causal_start >= 0;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (live && !direct) p.part_ml[rec] = make_float2(ref, sum);
+    if (live && !direct) p.part_ml[record + pair] = make_float2(ref, sum);
+    // O by way of shared memory (the converted chunks' space, once both slots are done with it), so
+    // that a warp writes whole rows.
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    float* o_s = reinterpret_cast<float*>(ring16 + warp * 16384);  // 32 rows x 512 B
+    const float inv = !direct ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll 1
     for (int q4 = 0; q4 < 4; ++q4) {
       float ov[32];
       if (n > 0) tmem_ld32(tO + q4 * 32, ov);
-      if (!live) continue;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int f = q4 * 8 + i;
+        const bool any = n > 0 && sum != 0.f;
+        *reinterpret_cast<float4*>(o_s + lane * kHd + ((f ^ (lane & 7)) * 4)) =
+            make_float4(any ? ov[4 * i] * inv : 0.f, any ? ov[4 * i + 1] * inv : 0.f, any ? ov[4 * i + 2] * inv : 0.f,
+                        any ? ov[4 * i + 3] * inv : 0.f);
+      }
+    }
+    __syncwarp();
+    const uint32_t filled = __ballot_sync(0xffffffffu, live && (direct || sum != 0.f));
+#pragma unroll 4
+    for (int i = 0; i < 32; ++i) {
+      const int64_t to = __shfl_sync(0xffffffffu, pair, i);
+      if (!((filled >> i) & 1u)) continue;  // warp-uniform
+      const float4 v = *reinterpret_cast<const float4*>(o_s + i * kHd + ((lane ^ (i & 7)) * 4));
       if (direct) {
-        T* out = static_cast<T*>(p.out) + pair * kHd + q4 * 32;
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          T v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = from_f32<T>(sum == 0.f ? 0.f : ov[i + e] * inv);
-          *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<const uint4*>(v);
-        }
-      } else if (sum != 0.f) {
-        float* out = p.part_o + rec * kHd + q4 * 32;
-#pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4*>(out + i) = make_float4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
+        T t[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + to * kHd + lane * 4) = *reinterpret_cast<const uint2*>(t);
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (record + to) * kHd + lane * 4) = v;
       }
     }
   }
