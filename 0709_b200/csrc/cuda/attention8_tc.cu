@@ -27,9 +27,10 @@ constexpr int kBytes8 = kChunk * kHd * 2;      // K | V codes
 constexpr int kHalf16 = kChunk * 128;          // 64 keys x 64 dimensions of fp16
 constexpr int kBytes16 = 4 * kHalf16;          // K halves | V halves
 constexpr int kBytesQ = 128 * kHd * 2;         // two halves of 128 rows x 128 B
+static_assert(256 * (kHd * 4 + 16) <= kStages8 * kBytes8 + 4 * kBytes16, "the output rows reuse the chunks' space");
 static_assert(kBytesQ == kBytes16, "slot 1's own Q takes the place of the fourth converted chunk");
 constexpr int kThreads = 608;
-constexpr int kSmem = 1024 + kStages8 * kBytes8 + 4 * kBytes16 + kBytesQ + (kStages8 + 4) * 128 + 256;
+constexpr int kSmem = 1024 + kStages8 * kBytes8 + 4 * kBytes16 + kBytesQ + (kStages8 + 4) * 128 + 256 + 256;
 constexpr uint32_t kColO = 256;
 constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
 }  // namespace
@@ -103,6 +104,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// Copy `bytes` (a multiple of 16) from shared to global memory, both 16-byte aligned; the wait returns
+// when this thread's copies have read their source.
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store_wait() {
+  asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
 // One lane of a converged warp, the same one every time.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -131,8 +142,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* s_full = empty16 + kStages16;  // [slot][buffer]
   uint64_t* p_full = s_full + 4;           // [2], 128 arrivals
   uint64_t* pv_done = p_full + 2;          // [2]
-  uint64_t* q_full = pv_done + 2;          // 256 arrivals
+  uint64_t* q_full = pv_done + 2;          // 512 arrivals
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
+  int8_t* q_exp = reinterpret_cast<int8_t*>(full8) + 256;  // [256] exponent that scaled each row of Q
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int h = blockIdx.x;
@@ -158,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&p_full[s], 128);
       mbar_init(&pv_done[s], 1);
     }
-    mbar_init(q_full, 256);
+    mbar_init(q_full, 512);
     fence_barrier_init();
     tma_prefetch_desc(&map);
   }
@@ -169,6 +181,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_trigger();  // after this CTA's TMEM allocation
+
+  // Q: warps 0-15 bring a sixteenth of the rows each, a row per load of the whole warp (a thread per row
+  // would touch 32 lines with every load), all loads in flight before anything else is read.
+  constexpr int kQRows = ksplit ? 8 : 16;
+  uint2 qraw[kQRows];
+  if (warp < 16) {
+    const int first = warp * kQRows;
+    int qm = (row0 + first) / G, qg = (row0 + first) - qm * G;
+    const uint2* src = reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + lane * 4);
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      qraw[i] = make_uint2(0, 0);
+      if (first + i < rows_cta) qraw[i] = src[(static_cast<int64_t>(qm) * p.Hq + h * G + qg) * (kHd / 4)];
+      if (++qg == G) {
+        qg = 0;
+        ++qm;
+      }
+    }
+  }
 
   // This split's chunks: up to the last key that any row of the CTA may see.
   const Attn8Shape sh = attn8_shape(p);
@@ -185,6 +216,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int c0 = static_cast<int>(blockIdx.y) * per;
   const int chunks = max(0, min(chunks_all, c0 + per) - c0);
   const int ps = 1 << p.page_shift;
+
+  if (warp < 16) {
+    // Each row scaled by a power of two so that its largest element is in [1, 2), as fp16, swizzled.
+#pragma unroll
+    for (int i = 0; i < kQRows; ++i) {
+      const T* e = reinterpret_cast<const T*>(&qraw[i]);
+      const float q[4] = {to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
+      const float am = fmaxf(max3(fabsf(q[0]), fabsf(q[1]), fabsf(q[2])), fabsf(q[3]));
+      const int e2 = row_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(am)));
+      const float down = __int_as_float((127 - e2) << 23);
+      const int row = warp * kQRows + i;
+      uint8_t* qs = row < 128 ? q_s : q1_s;
+      *reinterpret_cast<uint2*>(qs + (lane >> 4) * (kBytesQ / 2) + (lane & 1) * 8 +
+                                sw128_offset(row & 127, (lane & 15) >> 1)) =
+          make_uint2(pack_half2(q[0] * down, q[1] * down), pack_half2(q[2] * down, q[3] * down));
+      if (lane == 0) q_exp[row] = static_cast<int8_t>(e2);
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(q_full);
+  }
 
   if (warp == 16) {
     // ---- producer.  Lane l holds page and scales of 8 keys, l & 7, of chunk l >> 3 of a window of
@@ -342,46 +393,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       full = p.causal_start >= 0 ? len : min(p.row_full[m], len);
     }
     const int lim = min(len, end), sure = min(full, end);  // keys below `sure` are visible
-    // The warp's 32 rows of Q, each scaled by a power of two so that its largest element is in [1, 2),
-    // as fp16 in the swizzled layout.  A row is read by the whole warp (a thread per row touches 32
-    // lines with every load: 16,000 cycles for the CTA's rows), lane i keeps row i's factor.
-    int e2 = 0;
-    {
-      uint8_t* qs = slot == 0 ? q_s : q1_s;
-      const int first = (ksplit ? 0 : slot * 128) + (warp & 3) * 32;
-#pragma unroll 1
-      for (int i0 = 0; i0 < 32; i0 += 16) {
-        uint2 w[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int rr = row0 + first + i0 + i;
-          w[i] = make_uint2(0, 0);
-          if (first + i0 + i < rows_cta)
-            w[i] = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) +
-                                                   (static_cast<int64_t>(rr / G) * p.Hq + h * G + rr % G) * kHd + lane * 4);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const T* e = reinterpret_cast<const T*>(&w[i]);
-          const float q[4] = {to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
-          uint32_t ab = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) ab = max(ab, __float_as_uint(q[k]) & 0x7fffffffu);
-          const int x2 = row_exponent(__reduce_max_sync(0xffffffffu, ab));
-          const float down = __int_as_float((127 - x2) << 23);
-          if (lane == i0 + i) e2 = x2;
-          if (slot == 0 || !ksplit) {
-            const int row = (warp & 3) * 32 + i0 + i;
-            *reinterpret_cast<uint2*>(qs + (lane >> 4) * (kBytesQ / 2) + sw128_offset(row, (lane & 15) >> 1) +
-                                      (lane & 1) * 8) =
-                make_uint2(pack_half2(q[0] * down, q[1] * down), pack_half2(q[2] * down, q[3] * down));
-          }
-        }
-      }
-    }
+    mbar_wait(q_full, 0, p.err);
+    const int e2 = q_exp[r];
     const float fac = p.scale_log2 * __int_as_float((127 + e2) << 23);
-    fence_proxy_async_smem();
-    mbar_arrive(q_full);
 
     const int n = ksplit ? (chunks + 1 - slot) / 2 : chunks;
     float ref = -INFINITY, sum = 0.f;
@@ -469,38 +483,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int64_t record = (ksplit ? 2 * blockIdx.y + slot : blockIdx.y) * pairs;
     const bool direct = p.causal_start >= 0;
     if (live && !direct) p.part_ml[record + pair] = make_float2(ref, sum);
-    // O by way of shared memory (the converted chunks' space, once both slots are done with it), so
-    // that a warp writes whole rows.
+    // O by way of shared memory (the chunks' space, once both slots are done with it): a thread lays its
+    // row down and copies it out as one bulk transfer.  Rows are padded by 16 bytes against bank conflicts.
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    float* o_s = reinterpret_cast<float*>(ring16 + warp * 16384);  // 32 rows x 512 B
-    const float inv = !direct ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+    constexpr int kRowOut = kHd * 4 + 16;
+    uint8_t* row_s = ring8 + tid * kRowOut;
+    const bool any = n > 0 && sum != 0.f;
+    const float inv = !any ? 0.f : direct ? 1.f / sum : 1.f;
 #pragma unroll 1
     for (int q4 = 0; q4 < 4; ++q4) {
       float ov[32];
       if (n > 0) tmem_ld32(tO + q4 * 32, ov);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int f = q4 * 8 + i;
-        const bool any = n > 0 && sum != 0.f;
-        *reinterpret_cast<float4*>(o_s + lane * kHd + ((f ^ (lane & 7)) * 4)) =
-            make_float4(any ? ov[4 * i] * inv : 0.f, any ? ov[4 * i + 1] * inv : 0.f, any ? ov[4 * i + 2] * inv : 0.f,
-                        any ? ov[4 * i + 3] * inv : 0.f);
-      }
-    }
-    __syncwarp();
-    const uint32_t filled = __ballot_sync(0xffffffffu, live && (direct || sum != 0.f));
-#pragma unroll 4
-    for (int i = 0; i < 32; ++i) {
-      const int64_t to = __shfl_sync(0xffffffffu, pair, i);
-      if (!((filled >> i) & 1u)) continue;  // warp-uniform
-      const float4 v = *reinterpret_cast<const float4*>(o_s + i * kHd + ((lane ^ (i & 7)) * 4));
       if (direct) {
-        T t[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + to * kHd + lane * 4) = *reinterpret_cast<const uint2*>(t);
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          T t[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[e] = from_f32<T>(any ? ov[i + e] * inv : 0.f);
+          *reinterpret_cast<uint4*>(row_s + (q4 * 32 + i) * 2) = *reinterpret_cast<const uint4*>(t);
+        }
       } else {
-        *reinterpret_cast<float4*>(p.part_o + (record + to) * kHd + lane * 4) = v;
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          *reinterpret_cast<float4*>(row_s + (q4 * 32 + i) * 4) = make_float4(ov[i], ov[i + 1], ov[i + 2], ov[i + 3]);
       }
     }
+    fence_proxy_async_smem();
+    if (live && (direct || any)) {
+      void* to = direct ? static_cast<void*>(static_cast<T*>(p.out) + pair * kHd)
+                        : static_cast<void*>(p.part_o + (record + pair) * kHd);
+      bulk_store(to, row_s, direct ? kHd * 2 : kHd * 4);
+    }
+    bulk_store_wait();
   }
   tc_fence_before();
   __syncthreads();
