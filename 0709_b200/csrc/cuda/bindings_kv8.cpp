@@ -66,7 +66,7 @@ torch::Tensor kv8_append(torch::Tensor qkv, torch::Tensor table, torch::Tensor p
               "the rotary table must be contiguous fp32 [positions, 128] on the cache's device");
   check_int(pos, data, "positions", M);
   check_int(slots, data, "slots", M);
-  TORCH_CHECK(M < (int64_t{1} << 31) && (Hq + 3) / 4 + Hkv <= 65535, "kv8 append size");
+  TORCH_CHECK(M * (Hq + Hkv) < (int64_t{1} << 31), "kv8 append size");
   const bool bf16 = t == torch::kFloat32 ? out_bf16 != 0 : t == torch::kBFloat16;
   const c10::cuda::CUDAGuard guard(data.device());
   auto q = torch::empty({M, Hq, 128}, qkv.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf));

@@ -110,61 +110,43 @@ __device__ __forceinline__ void store4(O* p, const float* x) {
   *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
 }
 
-// grid (M, ceil(Hq / 4) + Hkv), 128 threads.  Query blocks: one warp per head.  KV blocks: the first
-// row of the batch that writes a page (the others leave at once) handles all of the page's rows for
-// one kv head, so each page and head has one writer and no order of blocks matters; a row whose
-// predecessor writes the same page -- 15 of 16 in a prompt -- leaves without a scan of the slots.
-template <typename T, typename O>
-__global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
+// One kv head of `page`, which row m writes, if m is the first row of the batch to write it: all of the
+// page's rows.  So each page and head has one writer and no order of blocks matters.
+template <typename T>
+__device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int page, int h) {
   __shared__ int owner[kMaxPage];  // row that writes slot o, -1: none
   __shared__ uint32_t amax_s[2];
   __shared__ int follower;
-  pdl_wait();
-  pdl_trigger();
-  const int m = blockIdx.x;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int qblocks = (p.Hq + 3) / 4;
   const T* qkv = static_cast<const T*>(p.qkv);
-  if (static_cast<int>(blockIdx.y) < qblocks) {
-    const int head = blockIdx.y * 4 + warp;
-    if (head >= p.Hq) return;
-    const int pos = p.pos[m];
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
-    if (pos >= 0 && pos < p.max_pos)
-      rotate4<T>(qkv + m * p.ld + head * kHd, p.table + static_cast<int64_t>(pos) * kHd, lane, y);
-    else if (lane == 0)
-      set_error(p.err, kErrBadIndex);
-    store4<O>(static_cast<O*>(p.q_out) + (static_cast<int64_t>(m) * p.Hq + head) * kHd + lane * 4, y);
-    return;
-  }
-  const int h = blockIdx.y - qblocks;
-  const int slot = p.slots[m];
-  const int page = slot >> p.page_shift;
   const int ps = 1 << p.page_shift;
-  if (slot < 0 || page >= p.num_pages) {
-    if (tid == 0) set_error(p.err, kErrBadIndex);
-    return;
-  }
-  if (m > 0) {
-    const int before = p.slots[m - 1];
-    if (before >= 0 && (before >> p.page_shift) == page) return;
-  }
+  __syncthreads();  // a page before this one may still be in use
   if (tid < kMaxPage) owner[tid] = -1;
   if (tid < 2) amax_s[tid] = 0;
   if (tid == 0) follower = 0;
   __syncthreads();
-  for (int j = tid; j < p.M; j += 128) {
-    const int s = p.slots[j];
+  auto note = [&](int j, int s) {
     if (s >= 0 && (s >> p.page_shift) == page) {
       if (j < m) follower = 1;
       atomicMax(&owner[s & (ps - 1)], j);
     }
+  };
+  const int vec = (reinterpret_cast<uintptr_t>(p.slots) & 15) == 0 ? p.M >> 2 : 0;
+#pragma unroll 4
+  for (int j = tid; j < vec; j += 128) {
+    const int4 s = reinterpret_cast<const int4*>(p.slots)[j];
+    note(4 * j, s.x);
+    note(4 * j + 1, s.y);
+    note(4 * j + 2, s.z);
+    note(4 * j + 3, s.w);
   }
+  for (int j = 4 * vec + tid; j < p.M; j += 128) note(j, p.slots[j]);
   float* scale = p.scale + (static_cast<int64_t>(page) * 2) * p.Hkv + h;
   const float old_k = scale[0], old_v = scale[p.Hkv];
   __syncthreads();
   if (follower) return;
   // Largest magnitudes of the new rows; a row that cannot be stored is reported and left out.
+#pragma unroll 4
   for (int o = warp; o < ps; o += 4) {
     const int r = owner[o];
     if (r < 0) continue;  // warp-uniform
@@ -202,6 +184,7 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
   uint32_t* kd = reinterpret_cast<uint32_t*>(p.data) +
                  ((static_cast<int64_t>(page) * 2) * p.Hkv + h) * ps * (kHd / 4) + lane;
   uint32_t* vd = kd + static_cast<int64_t>(p.Hkv) * ps * (kHd / 4);
+#pragma unroll 2
   for (int o = warp; o < ps; o += 4) {
     const int r = owner[o];
     uint32_t* ko = kd + o * (kHd / 4);
@@ -224,6 +207,53 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
   if (tid == 0) {
     scale[0] = new_k;
     scale[p.Hkv] = new_v;
+  }
+}
+
+// 128 threads.  The first q_blocks blocks rotate Q, q_per_warp (row, head) pairs per warp; the others
+// take kv_rows consecutive rows of one kv head each and write the pages that these rows start.
+template <typename T, typename O>
+__global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
+  pdl_wait();
+  pdl_trigger();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (static_cast<int>(blockIdx.x) < p.q_blocks) {
+    const int64_t first = (static_cast<int64_t>(blockIdx.x) * 4 + warp) * p.q_per_warp;
+    const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
+    int m = static_cast<int>(first / p.Hq), head = static_cast<int>(first - static_cast<int64_t>(m) * p.Hq);
+#pragma unroll 4
+    for (int i = 0; i < p.q_per_warp; ++i) {
+      if (first + i >= pairs) break;
+      const int pos = p.pos[m];
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      if (pos >= 0 && pos < p.max_pos)
+        rotate4<T>(static_cast<const T*>(p.qkv) + m * p.ld + head * kHd, p.table + static_cast<int64_t>(pos) * kHd,
+                   lane, y);
+      else if (lane == 0)
+        set_error(p.err, kErrBadIndex);
+      store4<O>(static_cast<O*>(p.q_out) + (first + i) * kHd + lane * 4, y);
+      if (++head == p.Hq) {
+        head = 0;
+        ++m;
+      }
+    }
+    return;
+  }
+  const int b = blockIdx.x - p.q_blocks;
+  const int h = b % p.Hkv, m0 = b / p.Hkv * p.kv_rows;
+  // The rows whose predecessor writes another page (one of 16 in a prompt) may be the first of theirs.
+  const int m = m0 + lane;
+  const bool mine = lane < p.kv_rows && m < p.M;
+  const int slot = mine ? p.slots[m] : 0, before = mine && m > 0 ? p.slots[m - 1] : -1;
+  const int page = slot >> p.page_shift;
+  const bool good = slot >= 0 && page < p.num_pages;
+  if (!good) set_error(p.err, kErrBadIndex);
+  uint32_t todo =
+      __ballot_sync(0xffffffffu, mine && good && !(before >= 0 && (before >> p.page_shift) == page));
+  while (todo) {
+    const int i = __ffs(todo) - 1;
+    todo &= todo - 1;
+    append_page<T>(p, m0 + i, __shfl_sync(0xffffffffu, page, i), h);
   }
 }
 
@@ -372,9 +402,17 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-cudaError_t launch_kv8_append(const Kv8AppendParams& p, cudaStream_t st) {
-  if (p.M == 0) return cudaSuccess;
-  const dim3 grid(p.M, (p.Hq + 3) / 4 + p.Hkv);
+cudaError_t launch_kv8_append(const Kv8AppendParams& params, cudaStream_t st) {
+  if (params.M == 0) return cudaSuccess;
+  // Few rows: every (row, head) on a warp of its own, for latency.  Many: blocks of one such piece each
+  // spend their time starting (98 us for 5001 rows); 8 pairs per warp and 16 rows per page block.
+  Kv8AppendParams p = params;
+  p.q_per_warp = p.M > 64 ? 8 : 1;
+  p.kv_rows = p.M > 64 ? 16 : 1;
+  const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
+  const int64_t per_block = 4 * p.q_per_warp;
+  p.q_blocks = static_cast<int>((pairs + per_block - 1) / per_block);
+  const dim3 grid(p.q_blocks + (p.M + p.kv_rows - 1) / p.kv_rows * p.Hkv);
   if (p.in_type == kKv8Bf16) return launch_k(kv8_append_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, st, p);
   if (p.in_type == kKv8F16) return launch_k(kv8_append_kernel<__half, __half>, grid, dim3(128), 0, st, p);
   if (p.out_bf16) return launch_k(kv8_append_kernel<float, __nv_bfloat16>, grid, dim3(128), 0, st, p);

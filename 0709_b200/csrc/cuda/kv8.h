@@ -25,6 +25,7 @@ struct Kv8AppendParams {
   int64_t ld;
   int M, Hq, Hkv, page_shift, num_pages, max_pos;
   int in_type, out_bf16;
+  int q_blocks, q_per_warp, kv_rows;  // launch shape, filled in by the launch
 };
 cudaError_t launch_kv8_append(const Kv8AppendParams& p, cudaStream_t st);
 
