@@ -80,25 +80,26 @@ __device__ __forceinline__ float diff_of_products(float a, float b, float c, flo
   return fmaf(a, b, -cd) + err;
 }
 
-// Lane l's four rotated values, dimensions 4 l .. 4 l + 3, of the head at x (rotate-half pairing:
-// dimension i < 64 pairs with i + 64).
-template <typename T>
-__device__ __forceinline__ void rotate4(const T* x, const float* cs, int lane, float* y) {
-  const int i = (lane & 15) * 4;
+// Dimensions i .. i + 3 and 64 + i .. 64 + i + 3 of the head at x, rotated (rotate-half pairing:
+// dimension i < 64 pairs with i + 64).  kExact: the rounding that follows is the coarse one of e4m3.
+template <typename T, bool kExact>
+__device__ __forceinline__ void rotate8(const T* x, const float* cs, int i, float* y) {
   float a[4], b[4], c[4], s[4];
   load4<T>(x + i, a);
   load4<T>(x + 64 + i, b);
   load4<float>(cs + i, c);
   load4<float>(cs + 64 + i, s);
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    y[e] = lane < 16 ? diff_of_products(a[e], c[e], b[e], s[e]) : diff_of_products(b[e], c[e], -a[e], s[e]);
+  for (int e = 0; e < 4; ++e) {
+    y[e] = kExact ? diff_of_products(a[e], c[e], b[e], s[e]) : a[e] * c[e] - b[e] * s[e];
+    y[4 + e] = kExact ? diff_of_products(b[e], c[e], -a[e], s[e]) : b[e] * c[e] + a[e] * s[e];
+  }
 }
 
-__device__ __forceinline__ uint32_t abs_bits_max4(const float* x) {
+__device__ __forceinline__ uint32_t abs_bits_max8(const float* x) {
   uint32_t m = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
+  for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
   return m;
 }
 
@@ -110,6 +111,16 @@ __device__ __forceinline__ void store4(O* p, const float* x) {
   *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(v);
 }
 
+// Row r's k (rotated) and v of kv head h: this lane of 16 holds k dimensions i .. i + 3, 64 + i .. 64 + i + 3
+// and v dimensions 2 i .. 2 i + 7, i = 4 * (lane & 15).
+template <typename T>
+__device__ __forceinline__ void load_kv8(const Kv8AppendParams& p, int r, int pos, int h, int i, float* k, float* v) {
+  const T* row = static_cast<const T*>(p.qkv) + r * p.ld;
+  rotate8<T, true>(row + (p.Hq + h) * kHd, p.table + static_cast<int64_t>(pos) * kHd, i, k);
+  load4<T>(row + (p.Hq + p.Hkv + h) * kHd + 2 * i, v);
+  load4<T>(row + (p.Hq + p.Hkv + h) * kHd + 2 * i + 4, v + 4);
+}
+
 // One kv head of `page`, which row m writes, if m is the first row of the batch to write it: all of the
 // page's rows.  So each page and head has one writer and no order of blocks matters.
 template <typename T>
@@ -118,7 +129,6 @@ __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int
   __shared__ uint32_t amax_s[2];
   __shared__ int follower;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const T* qkv = static_cast<const T*>(p.qkv);
   const int ps = 1 << p.page_shift;
   __syncthreads();  // a page before this one may still be in use
   if (tid < kMaxPage) owner[tid] = -1;
@@ -145,32 +155,37 @@ __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int
   const float old_k = scale[0], old_v = scale[p.Hkv];
   __syncthreads();
   if (follower) return;
-  // Largest magnitudes of the new rows; a row that cannot be stored is reported and left out.
-#pragma unroll 4
-  for (int o = warp; o < ps; o += 4) {
-    const int r = owner[o];
-    if (r < 0) continue;  // warp-uniform
-    const int pos = p.pos[r];
-    bool ok = pos >= 0 && pos < p.max_pos;
-    int code = kErrBadIndex;
-    if (ok) {
-      float k[4], v[4];
-      const T* row = qkv + r * p.ld;
-      rotate4<T>(row + (p.Hq + h) * kHd, p.table + static_cast<int64_t>(pos) * kHd, lane, k);
-      load4<T>(row + (p.Hq + p.Hkv + h) * kHd + lane * 4, v);
-      const uint32_t ak = __reduce_max_sync(0xffffffffu, abs_bits_max4(k));
-      const uint32_t av = __reduce_max_sync(0xffffffffu, abs_bits_max4(v));
-      ok = kv8_storable(ak) && kv8_storable(av);
-      code = kErrNonFinite;
-      if (ok && lane == 0) {
-        atomicMax(&amax_s[0], ak);
-        atomicMax(&amax_s[1], av);
-      }
+  // Largest magnitudes of the new rows, 16 lanes to a row; a row that cannot be stored is reported and
+  // left out.
+  const int i = (lane & 15) * 4, sub = lane >> 4;
+  uint32_t ak = 0, av = 0;
+#pragma unroll 2
+  for (int o2 = warp * 2; o2 < ps; o2 += 8) {
+    const int o = o2 + sub, r = owner[o];
+    const int pos = r >= 0 ? p.pos[r] : -1;
+    const bool in = pos >= 0 && pos < p.max_pos;
+    uint32_t lk = 0, lv = 0;
+    if (in) {
+      float k[8], v[8];
+      load_kv8<T>(p, r, pos, h, i, k, v);
+      lk = abs_bits_max8(k);
+      lv = abs_bits_max8(v);
     }
-    if (!ok && lane == 0) {
-      set_error(p.err, code);
+    const uint32_t fine = __ballot_sync(0xffffffffu, kv8_storable(lk) && kv8_storable(lv)) >> (16 * sub);
+    const bool ok = in && (fine & 0xffffu) == 0xffffu;
+    if (ok) {
+      ak = max(ak, lk);
+      av = max(av, lv);
+    } else if (r >= 0 && (lane & 15) == 0) {
+      set_error(p.err, in ? kErrNonFinite : kErrBadIndex);
       owner[o] = -1;
     }
+  }
+  ak = __reduce_max_sync(0xffffffffu, ak);
+  av = __reduce_max_sync(0xffffffffu, av);
+  if (lane == 0) {
+    atomicMax(&amax_s[0], ak);
+    atomicMax(&amax_s[1], av);
   }
   __syncthreads();
   const bool anew = owner[0] >= 0;
@@ -181,27 +196,30 @@ __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int
   const float new_k = anew ? need_k : fmaxf(old_k, need_k);
   const float new_v = anew ? need_v : fmaxf(old_v, need_v);
   const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
-  uint32_t* kd = reinterpret_cast<uint32_t*>(p.data) +
-                 ((static_cast<int64_t>(page) * 2) * p.Hkv + h) * ps * (kHd / 4) + lane;
+  uint32_t* kd = reinterpret_cast<uint32_t*>(p.data) + ((static_cast<int64_t>(page) * 2) * p.Hkv + h) * ps * (kHd / 4);
   uint32_t* vd = kd + static_cast<int64_t>(p.Hkv) * ps * (kHd / 4);
 #pragma unroll 2
-  for (int o = warp; o < ps; o += 4) {
-    const int r = owner[o];
-    uint32_t* ko = kd + o * (kHd / 4);
-    uint32_t* vo = vd + o * (kHd / 4);
+  for (int o2 = warp * 2; o2 < ps; o2 += 8) {
+    const int o = o2 + sub, r = owner[o];
+    uint32_t* ko = kd + o * (kHd / 4) + i / 4;  // words of dimensions i and 64 + i: 16 apart
+    uint2* vo = reinterpret_cast<uint2*>(vd + o * (kHd / 4) + i / 2);
     if (r >= 0) {
-      float k[4], v[4];
-      const T* row = qkv + r * p.ld;
-      rotate4<T>(row + (p.Hq + h) * kHd, p.table + static_cast<int64_t>(p.pos[r]) * kHd, lane, k);
-      load4<T>(row + (p.Hq + p.Hkv + h) * kHd + lane * 4, v);
-      *ko = kv8_encode4(k, inv_k);
-      *vo = kv8_encode4(v, inv_v);
+      float k[8], v[8];
+      load_kv8<T>(p, r, p.pos[r], h, i, k, v);
+      ko[0] = kv8_encode4(k, inv_k);
+      ko[16] = kv8_encode4(k + 4, inv_k);
+      *vo = make_uint2(kv8_encode4(v, inv_v), kv8_encode4(v + 4, inv_v));
     } else if (anew) {
-      *ko = 0;
-      *vo = 0;
+      ko[0] = 0;
+      ko[16] = 0;
+      *vo = make_uint2(0, 0);
     } else {
-      if (new_k > old_k && old_k > 0.f) *ko = kv8_rescale4(*ko, old_k * inv_k);
-      if (new_v > old_v && old_v > 0.f) *vo = kv8_rescale4(*vo, old_v * inv_v);
+      if (new_k > old_k && old_k > 0.f) {
+        ko[0] = kv8_rescale4(ko[0], old_k * inv_k);
+        ko[16] = kv8_rescale4(ko[16], old_k * inv_k);
+      }
+      if (new_v > old_v && old_v > 0.f)
+        *vo = make_uint2(kv8_rescale4(vo->x, old_v * inv_v), kv8_rescale4(vo->y, old_v * inv_v));
     }
   }
   if (tid == 0) {
@@ -218,24 +236,23 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (static_cast<int>(blockIdx.x) < p.q_blocks) {
-    const int64_t first = (static_cast<int64_t>(blockIdx.x) * 4 + warp) * p.q_per_warp;
-    const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
-    int m = static_cast<int>(first / p.Hq), head = static_cast<int>(first - static_cast<int64_t>(m) * p.Hq);
+    const uint32_t pairs = static_cast<uint32_t>(p.M) * p.Hq;  // below 2^31
+    uint32_t pair = (blockIdx.x * 4 + warp) * p.q_per_warp + (lane >> 4);  // 16 lanes each
+    const uint32_t stop = min(pairs, (blockIdx.x * 4 + warp + 1) * p.q_per_warp);
+    const int i = (lane & 15) * 4;
 #pragma unroll 4
-    for (int i = 0; i < p.q_per_warp; ++i) {
-      if (first + i >= pairs) break;
+    for (; pair < stop; pair += 2) {
+      const int m = pair / static_cast<uint32_t>(p.Hq), head = pair - m * p.Hq;
       const int pos = p.pos[m];
-      float y[4] = {0.f, 0.f, 0.f, 0.f};
+      float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (pos >= 0 && pos < p.max_pos)
-        rotate4<T>(static_cast<const T*>(p.qkv) + m * p.ld + head * kHd, p.table + static_cast<int64_t>(pos) * kHd,
-                   lane, y);
-      else if (lane == 0)
+        rotate8<T, false>(static_cast<const T*>(p.qkv) + m * p.ld + head * kHd,
+                          p.table + static_cast<int64_t>(pos) * kHd, i, y);
+      else if ((lane & 15) == 0)
         set_error(p.err, kErrBadIndex);
-      store4<O>(static_cast<O*>(p.q_out) + (first + i) * kHd + lane * 4, y);
-      if (++head == p.Hq) {
-        head = 0;
-        ++m;
-      }
+      O* out = static_cast<O*>(p.q_out) + static_cast<int64_t>(pair) * kHd + i;
+      store4<O>(out, y);
+      store4<O>(out + 64, y + 4);
     }
     return;
   }
@@ -407,7 +424,7 @@ cudaError_t launch_kv8_append(const Kv8AppendParams& params, cudaStream_t st) {
   // Few rows: every (row, head) on a warp of its own, for latency.  Many: blocks of one such piece each
   // spend their time starting (98 us for 5001 rows); 8 pairs per warp and 16 rows per page block.
   Kv8AppendParams p = params;
-  p.q_per_warp = p.M > 64 ? 8 : 1;
+  p.q_per_warp = p.M > 64 ? 8 : 2;
   p.kv_rows = p.M > 64 ? 16 : 1;
   const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
   const int64_t per_block = 4 * p.q_per_warp;
