@@ -532,8 +532,8 @@ __global__ void __launch_bounds__(128) attn8_merge_kernel(Attn8Params p) {
 template <typename T, int MT>
 static cudaError_t launch_split8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
   constexpr int smem = SplitCfg<MT>::kSmem;
-  const cudaError_t e =
-      cudaFuncSetAttribute(attn8_split_kernel<T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(attn8_split_kernel<T, MT>, smem, done);
   if (e != cudaSuccess) return e;
   const int rows = p.M * (p.Hq / p.Hkv);
   const dim3 grid(p.Hkv, p.splits, (rows + 16 * MT - 1) / (16 * MT));

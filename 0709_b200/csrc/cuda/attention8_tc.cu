@@ -523,8 +523,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <typename T, bool kSplitKeys>
 static cudaError_t launch_tc_typed(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
-  const cudaError_t e =
-      cudaFuncSetAttribute(attn8_tc_kernel<T, kSplitKeys>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(attn8_tc_kernel<T, kSplitKeys>, kSmem, done);
   if (e != cudaSuccess) return e;
   const int rows = p.M * (p.Hq / p.Hkv), tile = kSplitKeys ? 128 : 256;
   return launch_k(attn8_tc_kernel<T, kSplitKeys>, dim3(p.Hkv, p.tc_splits, (rows + tile - 1) / tile), dim3(kThreads),

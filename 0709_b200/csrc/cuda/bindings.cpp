@@ -67,33 +67,38 @@ CUtensorMapDataType tma_dtype(torch::ScalarType t) {
 
 // Row-major [outer, inner] with row stride `ld` elements; box {128 bytes, box_outer}, 128B swizzle
 // (64 elements of fp16/bf16, 128 of fp8).
-CUtensorMap map_2d(const torch::Tensor& t, int64_t inner, int64_t outer, int64_t ld, int box_outer) {
-  const bool byte = t.element_size() == 1;
+CUtensorMap map_rows(const void* ptr, torch::ScalarType type, int64_t inner, int64_t outer, int64_t ld, int box_outer) {
+  const int64_t esize = static_cast<int64_t>(c10::elementSize(type));
+  const bool byte = esize == 1;
   const uint32_t box_inner = byte ? 128 : 64;
   MapKey k{};
-  k.ptr = reinterpret_cast<uint64_t>(t.data_ptr());
+  k.ptr = reinterpret_cast<uint64_t>(ptr);
   k.d[0] = inner;
   k.d[1] = outer;
   k.d[2] = ld;
   k.box[0] = box_inner;
   k.box[1] = box_outer;
   k.rank = 2;
-  k.dtype = static_cast<int>(t.scalar_type());
+  k.dtype = static_cast<int>(type);
   std::lock_guard<std::mutex> g(g_map_mu);
   auto it = g_maps.find(k);
   if (it != g_maps.end()) return it->second;
   if (g_maps.size() > 8192) g_maps.clear();
   CUtensorMap m;
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
-  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * t.element_size()};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * esize)};
   cuuint32_t box[2] = {box_inner, static_cast<cuuint32_t>(box_outer)};
   cuuint32_t es[2] = {1, 1};
-  CUresult r = encode_fn()(&m, byte ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tma_dtype(t.scalar_type()), 2, t.data_ptr(), dims, strides, box, es,
-                           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  CUresult r = encode_fn()(&m, byte ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tma_dtype(type), 2, const_cast<void*>(ptr), dims,
+                           strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (2d) failed: ", static_cast<int>(r));
   g_maps.emplace(k, m);
   return m;
+}
+
+CUtensorMap map_2d(const torch::Tensor& t, int64_t inner, int64_t outer, int64_t ld, int box_outer) {
+  return map_rows(t.data_ptr(), t.scalar_type(), inner, outer, ld, box_outer);
 }
 
 // KV cache [L, NP, 2, Hkv, ps, hd] as 5-D {hd, ps, Hkv, 2, L*NP}; box {64, ps, 1, 1, 1}.
@@ -805,9 +810,8 @@ void gather_logprobs(torch::Tensor logits, torch::Tensor rows, torch::Tensor tok
 
 }  // namespace
 
-CUtensorMap map_kv8(const torch::Tensor& data) {
-  const int64_t rows = data.numel() / 128;
-  return map_2d(data, 128, rows, 128, static_cast<int>(std::min<int64_t>(data.size(-2), 16)));
+CUtensorMap map_kv8(const void* data, int64_t rows, int64_t ps) {
+  return map_rows(data, torch::kFloat8_e4m3fn, 128, rows, 128, static_cast<int>(std::min<int64_t>(ps, 16)));
 }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

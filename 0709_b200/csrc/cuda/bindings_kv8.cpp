@@ -16,20 +16,37 @@ namespace {
 
 constexpr double kLog2e = 1.4426950408889634;
 
-// data [.., pages, 2, Hkv, ps, 128] e4m3 with scale of the leading dimensions; returns log2(page size).
-int check_cache(const torch::Tensor& data, const torch::Tensor& scale, int64_t dim) {
-  TORCH_CHECK(data.is_cuda() && data.dim() == dim && data.is_contiguous() &&
+// A cache data [L, pages, 2, Hkv, ps, 128] e4m3 with scale [L, pages, 2, Hkv], or one of its layers.
+struct Cache8 {
+  uint8_t* data;
+  float* scale;
+  int64_t layers, pages, Hkv, ps;
+  int shift;  // log2(ps)
+};
+
+Cache8 check_cache(const torch::Tensor& data, const torch::Tensor& scale, int64_t layer = -1) {
+  TORCH_CHECK(data.is_cuda() && data.dim() == 6 && data.is_contiguous() &&
                   data.scalar_type() == torch::kFloat8_e4m3fn,
-              "the 8-bit cache must be a contiguous float8_e4m3fn CUDA tensor of ", dim, " dimensions");
-  TORCH_CHECK(data.size(-1) == 128 && data.size(-4) == 2, "the 8-bit cache kernels need [.., 2, Hkv, page, 128]");
-  const int64_t ps = data.size(-2);
+              "the 8-bit cache must be a contiguous float8_e4m3fn CUDA tensor [L, pages, 2, Hkv, page, 128]");
+  TORCH_CHECK(data.size(5) == 128 && data.size(2) == 2, "the 8-bit cache kernels need [L, pages, 2, Hkv, page, 128]");
+  const int64_t L = data.size(0), pages = data.size(1), Hkv = data.size(3), ps = data.size(4);
   TORCH_CHECK(ps == 8 || ps == 16 || ps == 32 || ps == 64, "the 8-bit cache kernels need pages of 8, 16, 32 or 64 slots");
   TORCH_CHECK(scale.scalar_type() == torch::kFloat32 && scale.is_contiguous() && scale.device() == data.device() &&
-                  scale.sizes() == data.sizes().slice(0, dim - 2),
+                  scale.sizes() == data.sizes().slice(0, 4),
               "the 8-bit cache needs one float32 scale per page, side and head on its device");
-  TORCH_CHECK(data.numel() / 128 < (int64_t{1} << 31) && data.size(-5) > 0 && data.size(-3) > 0, "8-bit cache size");
+  TORCH_CHECK(L > 0 && pages > 0 && Hkv > 0 && L <= 65535 && 2 * Hkv <= 65535 &&
+                  pages * 2 * Hkv * ps < (int64_t{1} << 31),
+              "a layer of the 8-bit cache holds fewer than 2^31 rows of 128 codes");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, "the 8-bit cache must be 16-byte aligned");
-  return ps == 8 ? 3 : ps == 16 ? 4 : ps == 32 ? 5 : 6;
+  TORCH_CHECK(layer >= -1 && layer < L, "layer ", layer, " of a cache of ", L);
+  Cache8 c{static_cast<uint8_t*>(data.data_ptr()), scale.data_ptr<float>(), L, pages, Hkv, ps,
+           ps == 8 ? 3 : ps == 16 ? 4 : ps == 32 ? 5 : 6};
+  if (layer >= 0) {
+    c.data += layer * pages * 2 * Hkv * ps * 128;
+    c.scale += layer * pages * 2 * Hkv;
+    c.layers = 1;
+  }
+  return c;
 }
 
 void check_int(const torch::Tensor& t, const torch::Tensor& like, const char* name, int64_t n = -1) {
@@ -47,13 +64,13 @@ void check_launch(cudaError_t e, const char* what) {
   TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
 }
 
-uint8_t* bytes(const torch::Tensor& t) { return static_cast<uint8_t*>(t.data_ptr()); }
-
 torch::Tensor kv8_append(torch::Tensor qkv, torch::Tensor table, torch::Tensor pos, torch::Tensor slots,
-                         torch::Tensor data, torch::Tensor scale, int64_t Hq, int64_t out_bf16, torch::Tensor err) {
-  const int shift = check_cache(data, scale, 5);
+                         torch::Tensor data, torch::Tensor scale, int64_t layer, int64_t Hq, bool out_bf16,
+                         torch::Tensor err) {
+  TORCH_CHECK(layer >= 0, "layer ", layer);
+  const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
-  const int64_t Hkv = data.size(2), M = qkv.size(0);
+  const int64_t Hkv = c.Hkv, M = qkv.size(0);
   const auto t = qkv.scalar_type();
   TORCH_CHECK(t == torch::kHalf || t == torch::kBFloat16 || t == torch::kFloat32, "qkv must be fp16, bf16 or fp32");
   TORCH_CHECK(qkv.device() == data.device() && qkv.dim() == 2 && Hq >= 1 && qkv.size(1) == (Hq + 2 * Hkv) * 128,
@@ -67,7 +84,7 @@ torch::Tensor kv8_append(torch::Tensor qkv, torch::Tensor table, torch::Tensor p
   check_int(pos, data, "positions", M);
   check_int(slots, data, "slots", M);
   TORCH_CHECK(M * (Hq + Hkv) < (int64_t{1} << 31), "kv8 append size");
-  const bool bf16 = t == torch::kFloat32 ? out_bf16 != 0 : t == torch::kBFloat16;
+  const bool bf16 = t == torch::kFloat32 ? out_bf16 : t == torch::kBFloat16;
   const c10::cuda::CUDAGuard guard(data.device());
   auto q = torch::empty({M, Hq, 128}, qkv.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf));
   atlas::Kv8AppendParams p{};
@@ -75,16 +92,16 @@ torch::Tensor kv8_append(torch::Tensor qkv, torch::Tensor table, torch::Tensor p
   p.table = table.data_ptr<float>();
   p.pos = pos.data_ptr<int>();
   p.slots = slots.data_ptr<int>();
-  p.data = bytes(data);
-  p.scale = scale.data_ptr<float>();
+  p.data = c.data;
+  p.scale = c.scale;
   p.q_out = q.data_ptr();
   p.err = err.data_ptr<int>();
   p.ld = qkv.stride(0);
   p.M = static_cast<int>(M);
   p.Hq = static_cast<int>(Hq);
   p.Hkv = static_cast<int>(Hkv);
-  p.page_shift = shift;
-  p.num_pages = static_cast<int>(data.size(0));
+  p.page_shift = c.shift;
+  p.num_pages = static_cast<int>(c.pages);
   p.max_pos = static_cast<int>(table.size(0));
   p.in_type = t == torch::kFloat32 ? atlas::kKv8F32 : t == torch::kBFloat16 ? atlas::kKv8Bf16 : atlas::kKv8F16;
   p.out_bf16 = bf16 ? 1 : 0;
@@ -94,7 +111,7 @@ torch::Tensor kv8_append(torch::Tensor qkv, torch::Tensor table, torch::Tensor p
 
 void kv8_copy_pages(torch::Tensor data, torch::Tensor scale, torch::Tensor plan, c10::optional<torch::Tensor> count,
                     torch::Tensor err) {
-  const int shift = check_cache(data, scale, 6);
+  const Cache8 c = check_cache(data, scale);
   check_err(err, data);
   check_int(plan, data, "the copy plan");
   TORCH_CHECK(plan.dim() == 2 && plan.size(1) == 3, "the copy plan must be [n, 3]");
@@ -102,48 +119,44 @@ void kv8_copy_pages(torch::Tensor data, torch::Tensor scale, torch::Tensor plan,
     check_int(*count, data, "the copy count");
     TORCH_CHECK(count->numel() >= 1, "the copy count must hold one value");
   }
-  TORCH_CHECK(data.size(0) <= 65535 && 2 * data.size(3) <= 65535, "kv8 copy size");
   const c10::cuda::CUDAGuard guard(data.device());
-  check_launch(atlas::launch_kv8_copy_pages(bytes(data), scale.data_ptr<float>(), plan.data_ptr<int>(),
+  check_launch(atlas::launch_kv8_copy_pages(c.data, c.scale, plan.data_ptr<int>(),
                                             count.has_value() ? count->data_ptr<int>() : nullptr,
-                                            static_cast<int>(plan.size(0)), static_cast<int>(data.size(0)),
-                                            static_cast<int>(data.size(1)), static_cast<int>(data.size(3)), shift,
+                                            static_cast<int>(plan.size(0)), static_cast<int>(c.layers),
+                                            static_cast<int>(c.pages), static_cast<int>(c.Hkv), c.shift,
                                             err.data_ptr<int>(), at::cuda::getCurrentCUDAStream()),
                "kv8_copy_pages");
 }
 
 void kv8_move_slots(torch::Tensor data, torch::Tensor scale, torch::Tensor src, torch::Tensor dst, torch::Tensor err) {
-  const int shift = check_cache(data, scale, 6);
+  const Cache8 c = check_cache(data, scale);
   check_err(err, data);
   check_int(src, data, "source slots");
   check_int(dst, data, "destination slots", src.numel());
   TORCH_CHECK(src.numel() <= atlas::kKv8MaxMoves, "at most ", atlas::kKv8MaxMoves, " slot moves per call, not ",
               src.numel());
-  TORCH_CHECK(2 * data.size(3) <= 65535, "kv8 move size");
   const c10::cuda::CUDAGuard guard(data.device());
-  check_launch(atlas::launch_kv8_move_slots(bytes(data), scale.data_ptr<float>(), src.data_ptr<int>(),
-                                            dst.data_ptr<int>(), static_cast<int>(src.numel()),
-                                            static_cast<int>(data.size(0)), static_cast<int>(data.size(1)),
-                                            static_cast<int>(data.size(3)), shift, err.data_ptr<int>(),
-                                            at::cuda::getCurrentCUDAStream()),
+  check_launch(atlas::launch_kv8_move_slots(c.data, c.scale, src.data_ptr<int>(), dst.data_ptr<int>(),
+                                            static_cast<int>(src.numel()), static_cast<int>(c.layers),
+                                            static_cast<int>(c.pages), static_cast<int>(c.Hkv), c.shift,
+                                            err.data_ptr<int>(), at::cuda::getCurrentCUDAStream()),
                "kv8_move_slots");
 }
 
-// One layer (data of 5 dimensions) -> [n, 2, Hkv, ps, 128]; a whole cache (6) -> [L, n, 2, Hkv, ps, 128].
-torch::Tensor kv8_read_pages(torch::Tensor data, torch::Tensor scale, torch::Tensor pages, bool bf16,
+// One layer -> [n, 2, Hkv, ps, 128]; the whole cache (layer -1) -> [L, n, 2, Hkv, ps, 128].
+torch::Tensor kv8_read_pages(torch::Tensor data, torch::Tensor scale, int64_t layer, torch::Tensor pages, bool bf16,
                              torch::Tensor err) {
-  const bool layers = data.dim() == 6;
-  const int shift = check_cache(data, scale, layers ? 6 : 5);
+  const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
   check_int(pages, data, "pages");
-  const int64_t L = layers ? data.size(0) : 1, n = pages.numel(), Hkv = data.size(-3), ps = data.size(-2);
-  TORCH_CHECK(L <= 65535 && 2 * Hkv <= 65535, "kv8 read size");
+  const int64_t n = pages.numel();
   const c10::cuda::CUDAGuard guard(data.device());
   const auto opt = data.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf);
-  auto out = layers ? torch::empty({L, n, 2, Hkv, ps, 128}, opt) : torch::empty({n, 2, Hkv, ps, 128}, opt);
-  check_launch(atlas::launch_kv8_read_pages(bytes(data), scale.data_ptr<float>(), pages.data_ptr<int>(),
-                                            out.data_ptr(), static_cast<int>(n), static_cast<int>(L),
-                                            static_cast<int>(data.size(-5)), static_cast<int>(Hkv), shift, bf16,
+  auto out = layer < 0 ? torch::empty({c.layers, n, 2, c.Hkv, c.ps, 128}, opt)
+                       : torch::empty({n, 2, c.Hkv, c.ps, 128}, opt);
+  check_launch(atlas::launch_kv8_read_pages(c.data, c.scale, pages.data_ptr<int>(), out.data_ptr(),
+                                            static_cast<int>(n), static_cast<int>(c.layers),
+                                            static_cast<int>(c.pages), static_cast<int>(c.Hkv), c.shift, bf16,
                                             err.data_ptr<int>(), at::cuda::getCurrentCUDAStream()),
                "kv8_read_pages");
   return out;
@@ -165,32 +178,32 @@ void pick_shape8(atlas::Attn8Params& p, int64_t rows, int64_t keys, int sms) {
   p.splits = static_cast<int>(most == 32 ? 2 * n : n);
 }
 
-void check_q8(torch::Tensor& q, const torch::Tensor& data, double softmax_scale) {
+void check_q8(torch::Tensor& q, const torch::Tensor& data, const Cache8& c, double softmax_scale) {
   TORCH_CHECK(q.device() == data.device() && q.dim() == 3 && q.size(2) == 128 &&
                   (q.scalar_type() == torch::kHalf || q.scalar_type() == torch::kBFloat16),
               "q must be fp16 or bf16 [M, Hq, 128] on the cache's device");
-  TORCH_CHECK(q.size(1) >= 1 && q.size(1) % data.size(2) == 0, "Hq must be a multiple of Hkv");
-  TORCH_CHECK(q.size(0) * q.size(1) / data.size(2) <= 65535 * 128, "attention8 takes at most 65535 * 128 query rows per kv head");
+  TORCH_CHECK(q.size(1) >= 1 && q.size(1) % c.Hkv == 0, "Hq must be a multiple of Hkv");
+  TORCH_CHECK(q.size(0) * (q.size(1) / c.Hkv) <= 65535 * 128,
+              "attention8 takes at most 65535 * 128 query rows per kv head");
   TORCH_CHECK(softmax_scale > 0 && std::isfinite(softmax_scale), "the softmax scale must be positive and finite");
   if (!q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0)
     q = q.clone(at::MemoryFormat::Contiguous);
 }
 
-atlas::Attn8Params params8(const torch::Tensor& q, const torch::Tensor& data, const torch::Tensor& scale, int shift,
-                           const torch::Tensor& out, const torch::Tensor& prefix_pages, double softmax_scale,
-                           const torch::Tensor& err) {
+atlas::Attn8Params params8(const torch::Tensor& q, const Cache8& c, const torch::Tensor& out,
+const torch::Tensor& prefix_pages, double softmax_scale, const torch::Tensor& err) {
   atlas::Attn8Params p{};
   p.q = q.data_ptr();
-  p.data = bytes(data);
-  p.scale = scale.data_ptr<float>();
+  p.data = c.data;
+  p.scale = c.scale;
   p.out = out.data_ptr();
   p.prefix_pages = prefix_pages.data_ptr<int>();
   p.err = err.data_ptr<int>();
   p.M = static_cast<int>(q.size(0));
   p.Hq = static_cast<int>(q.size(1));
-  p.Hkv = static_cast<int>(data.size(2));
-  p.page_shift = shift;
-  p.num_pages = static_cast<int>(data.size(0));
+  p.Hkv = static_cast<int>(c.Hkv);
+  p.page_shift = c.shift;
+  p.num_pages = static_cast<int>(c.pages);
   p.n_prefix = static_cast<int>(prefix_pages.numel());
   p.bf16 = q.scalar_type() == torch::kBFloat16;
   p.scale_log2 = static_cast<float>(softmax_scale * kLog2e);
@@ -198,14 +211,16 @@ atlas::Attn8Params params8(const torch::Tensor& q, const torch::Tensor& data, co
   return p;
 }
 
-std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data, torch::Tensor scale, c10::optional<torch::Tensor> dparams,
-                         int64_t shared_len, int64_t n_shared_pages, int64_t mask_base, torch::Tensor prefix_pages,
+std::pair<torch::Tensor, int64_t> attention8(
+                         torch::Tensor q, torch::Tensor data, torch::Tensor scale, int64_t layer,
+                         c10::optional<torch::Tensor> dparams, int64_t shared_len, int64_t n_shared_pages, int64_t mask_base, torch::Tensor prefix_pages,
                          torch::Tensor row_full, torch::Tensor row_len, torch::Tensor row_mask, torch::Tensor tail_pages,
                          double softmax_scale, int64_t max_keys, torch::Tensor err) {
-  const int shift = check_cache(data, scale, 5);
+  TORCH_CHECK(layer >= 0, "layer ", layer);
+  const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
-  check_q8(q, data, softmax_scale);
-  const int64_t M = q.size(0), Hq = q.size(1), Hkv = data.size(2);
+  check_q8(q, data, c, softmax_scale);
+  const int64_t M = q.size(0), Hq = q.size(1), Hkv = c.Hkv;
   check_int(prefix_pages, data, "prefix_pages");
   check_int(row_full, data, "row_full", M);
   check_int(row_len, data, "row_len", M);
@@ -214,7 +229,7 @@ std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data
               "row_mask must be contiguous int64 [M, words] on the cache's device");
   check_int(tail_pages, data, "tail_pages");
   TORCH_CHECK(tail_pages.dim() == 2 && tail_pages.size(0) == M, "tail_pages must be [M, T]");
-  TORCH_CHECK(shared_len >= 0 && n_shared_pages >= 0 && std::max(shared_len, n_shared_pages << shift) < (1 << 30),
+  TORCH_CHECK(shared_len >= 0 && n_shared_pages >= 0 && std::max(shared_len, n_shared_pages << c.shift) < (1 << 30),
               "shared_len and n_shared_pages must be positions below 2^30");
   if (dparams.has_value()) {
     check_int(*dparams, data, "the descriptor's device scalars");
@@ -223,7 +238,7 @@ std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data
   const c10::cuda::CUDAGuard guard(data.device());
   auto out = torch::empty({M, Hq * 128}, q.options());
   if (M == 0) return {out, 0};
-  atlas::Attn8Params p = params8(q, data, scale, shift, out, prefix_pages, softmax_scale, err);
+  atlas::Attn8Params p = params8(q, c, out, prefix_pages, softmax_scale, err);
   p.dparams = dparams.has_value() ? dparams->data_ptr<int>() : nullptr;
   p.shared_len = static_cast<int>(shared_len);
   p.n_shared_pages = static_cast<int>(n_shared_pages);
@@ -235,11 +250,11 @@ std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data
   p.mask_words = static_cast<int>(row_mask.size(1));
   p.tail_stride = static_cast<int>(tail_pages.size(1));
   // A captured call is sized for the longest context its graph may see (max_keys), an eager one for its own.
-  const int64_t keys = std::max<int64_t>({shared_len, n_shared_pages << shift, max_keys});
+  const int64_t keys = std::max<int64_t>({shared_len, n_shared_pages << c.shift, max_keys});
   CUtensorMap map{};
   if (keys > 0 || dparams.has_value()) {
     pick_shape8(p, M * (Hq / Hkv), keys, at::cuda::getCurrentDeviceProperties()->multiProcessorCount);
-    map = map_kv8(data);
+    map = map_kv8(c.data, c.pages * 2 * Hkv * c.ps, c.ps);
   }
   torch::Tensor parts;
   if (p.splits > 0) {
@@ -252,13 +267,14 @@ std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data
 }
 
 // Row m is at position start + m and sees the keys up to itself, all in prefix_pages.
-torch::Tensor attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tensor scale, torch::Tensor prefix_pages,
-                                int64_t start, double softmax_scale, torch::Tensor err) {
-  const int shift = check_cache(data, scale, 5);
+torch::Tensor attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tensor scale, int64_t layer,
+                                torch::Tensor prefix_pages, int64_t start, double softmax_scale, torch::Tensor err) {
+  TORCH_CHECK(layer >= 0, "layer ", layer);
+  const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
-  check_q8(q, data, softmax_scale);
+  check_q8(q, data, c, softmax_scale);
   check_int(prefix_pages, data, "prefix_pages");
-  const int64_t M = q.size(0), ps = data.size(3);
+  const int64_t M = q.size(0), ps = c.ps;
   TORCH_CHECK(start >= 0 && start + M < (1 << 30), "positions must be in [0, 2^30)");
   const int64_t n = (start + M + ps - 1) / ps;
   TORCH_CHECK(n <= prefix_pages.numel(), start + M, " positions need ", n, " pages of ", ps,
@@ -266,11 +282,11 @@ torch::Tensor attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tens
   const c10::cuda::CUDAGuard guard(data.device());
   auto out = torch::empty({M, q.size(1) * 128}, q.options());
   if (M == 0) return out;
-  atlas::Attn8Params p = params8(q, data, scale, shift, out, prefix_pages, softmax_scale, err);
+  atlas::Attn8Params p = params8(q, c, out, prefix_pages, softmax_scale, err);
   p.causal_start = static_cast<int>(start);
   p.shared_len = static_cast<int>(start + M);
   p.tc_splits = 1;
-  check_launch(atlas::launch_attention8_tc(map_kv8(data), p, at::cuda::getCurrentCUDAStream()), "attention8_causal");
+  check_launch(atlas::launch_attention8_tc(map_kv8(c.data, c.pages * 2 * c.Hkv * ps, ps), p, at::cuda::getCurrentCUDAStream()), "attention8_causal");
   return out;
 }
 

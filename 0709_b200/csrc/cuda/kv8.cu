@@ -449,8 +449,8 @@ cudaError_t launch_kv8_move_slots(uint8_t* data, float* scale, const int* src, c
   if (n == 0) return cudaSuccess;
   const size_t smem = static_cast<size_t>(n) * (kHd + 8);
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kv8_move_slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               kKv8MaxMoves * (kHd + 8));
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem(kv8_move_slots_kernel, kKv8MaxMoves * (kHd + 8), done);
     if (e != cudaSuccess) return e;
   }
   return launch_k(kv8_move_slots_kernel, dim3(layers, 2 * Hkv), dim3(256), smem, st, data, scale, src, dst, n,

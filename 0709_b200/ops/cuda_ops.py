@@ -311,14 +311,15 @@ class CudaOps:
     def rope_qkv_append8(self, qkv, table, positions, slots, kv_layer, num_heads, num_kv_heads, out_dtype=None):
         """Rotate q/k, round k and v into the layer's pages at ``slots`` (one launch); returns q [M, Hq, 128] in
         ``qkv``'s dtype, or in ``out_dtype`` (fp16 by default) when ``qkv`` is fp32."""
-        if num_kv_heads != kv_layer.data.shape[-3]:
-            raise ValueError(f"{num_kv_heads} kv heads for a cache of {kv_layer.data.shape[-3]}")
+        cache = kv_layer.cache
+        if num_kv_heads != cache.data.shape[3]:
+            raise ValueError(f"{num_kv_heads} kv heads for a cache of {cache.data.shape[3]}")
         if out_dtype is None:
             out_dtype = torch.float16 if qkv.dtype == torch.float32 else qkv.dtype
         if out_dtype not in (torch.float16, torch.bfloat16) or qkv.dtype not in (out_dtype, torch.float32):
             raise TypeError(f"rope_qkv_append8 writes q in fp16 or bf16, not {out_dtype} from {qkv.dtype}")
-        q = self.ext.kv8_append(qkv, table, self._int32(positions), self._int32(slots), kv_layer.data, kv_layer.scale,
-                                num_heads, out_dtype == torch.bfloat16, self.err)
+        q = self.ext.kv8_append(qkv, table, self._int32(positions), self._int32(slots), cache.data, cache.scale,
+                                kv_layer.index, num_heads, out_dtype == torch.bfloat16, self.err)
         counters.launches(1)
         return q
 
@@ -327,8 +328,8 @@ class CudaOps:
         dtype.  A row that sees no key answers zero."""
         scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
         out, launches = self.ext.attention8(
-            q, kv_layer.data, kv_layer.scale, getattr(desc, "_dparams", None), desc.shared_len, desc.n_shared_pages,
-            desc.mask_base, desc.prefix_pages, desc.row_full, desc.row_len, desc.row_mask, desc.tail_pages, scale,
+            q, kv_layer.cache.data, kv_layer.cache.scale, kv_layer.index, getattr(desc, "_dparams", None),
+            desc.shared_len, desc.n_shared_pages, desc.mask_base, desc.prefix_pages, desc.row_full, desc.row_len, desc.row_mask, desc.tail_pages, scale,
             getattr(desc, "_max_keys", 0), self.err,
         )
         counters.launches(launches)
@@ -338,8 +339,8 @@ class CudaOps:
         """Attention of a prefill chunk at positions ``causal_start ..`` whose own keys are in the 8-bit cache
         already; the descriptor gives the page list."""
         scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-        out = self.ext.attention8_causal(q, kv_layer.data, kv_layer.scale, desc.prefix_pages, int(causal_start), scale,
-                                         self.err)
+        out = self.ext.attention8_causal(q, kv_layer.cache.data, kv_layer.cache.scale, kv_layer.index,
+                                         desc.prefix_pages, int(causal_start), scale, self.err)
         counters.launches(1)
         return out
 
@@ -363,7 +364,10 @@ class CudaOps:
         """The values of ``pages`` in fp16 or bf16: [n, 2, Hkv, page, 128] of a layer, [L, n, ...] of a cache."""
         if dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"kv8_read_pages gives fp16 or bf16, not {dtype}")
-        out = self.ext.kv8_read_pages(cache.data, cache.scale, self._int32(pages), dtype == torch.bfloat16, self.err)
+        layer = getattr(cache, "index", -1)  # a layer of a cache, or all of it
+        whole = cache if layer < 0 else cache.cache
+        out = self.ext.kv8_read_pages(whole.data, whole.scale, layer, self._int32(pages), dtype == torch.bfloat16,
+                                      self.err)
         counters.launches(1)
         return out
 

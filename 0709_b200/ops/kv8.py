@@ -32,24 +32,12 @@ EXP_MIN, EXP_MAX = -40, 56
 
 
 @dataclass
-class Kv8Layer:
-    """One layer's view: ``data [pages, 2, kv_heads, page_size, head_dim]``, ``scale [pages, 2, kv_heads]``."""
-
-    data: torch.Tensor
-    scale: torch.Tensor
-
-    def values(self) -> torch.Tensor:
-        """Every element in fp32."""
-        return self.data.float() * self.scale[..., None, None]
-
-
-@dataclass
 class Kv8Cache:
     data: torch.Tensor
     scale: torch.Tensor
 
-    def layer(self, index: int) -> Kv8Layer:
-        return Kv8Layer(self.data[index], self.scale[index])
+    def layer(self, index: int) -> "Kv8Layer":
+        return Kv8Layer(self, index)
 
     def __getitem__(self, index: int) -> Kv8Layer:
         return self.layer(index)
@@ -57,6 +45,32 @@ class Kv8Cache:
     @property
     def nbytes(self) -> int:
         return self.data.numel() + 4 * self.scale.numel()
+
+
+@dataclass
+class Kv8Layer:
+    """One layer of a cache (a name for it: the kernels take the cache and the index, so no view is made per call)."""
+
+    cache: Kv8Cache
+    index: int
+
+    def __post_init__(self) -> None:
+        if not 0 <= self.index < self.cache.data.shape[0]:
+            raise IndexError(f"layer {self.index} of a cache of {self.cache.data.shape[0]}")
+
+    @property
+    def data(self) -> torch.Tensor:
+        """[pages, 2, kv_heads, page_size, head_dim]"""
+        return self.cache.data[self.index]
+
+    @property
+    def scale(self) -> torch.Tensor:
+        """[pages, 2, kv_heads]"""
+        return self.cache.scale[self.index]
+
+    def values(self) -> torch.Tensor:
+        """Every element in fp32."""
+        return self.data.float() * self.scale[..., None, None]
 
 
 def empty_cache(layers: int, pages: int, kv_heads: int, page_size: int, head_dim: int, device=None) -> Kv8Cache:

@@ -227,7 +227,7 @@ def kv8_read_pages(cache: kv8.Kv8Cache | kv8.Kv8Layer, pages: torch.Tensor, dtyp
     largest finite value of ``dtype``)."""
     idx = pages.long()
     data, scale = cache.data.view(torch.uint8), cache.scale
-    if data.dim() == 6:
+    if isinstance(cache, kv8.Kv8Cache):
         data, scale = data[:, idx], scale[:, idx]
     else:
         data, scale = data[idx], scale[idx]
