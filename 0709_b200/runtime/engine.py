@@ -57,11 +57,7 @@ class LlamaEngine:
         self.page_size = int(page_size)
         self.num_pages = int(num_pages)
         c = self.cfg
-        self.kv = torch.zeros(
-            (c.num_layers, self.num_pages, 2, c.num_kv_heads, self.page_size, c.head_dim),
-            dtype=self.dtype,
-            device=self.device,
-        )
+        self.kv = self._new_cache()
         self.rope = rope_table(c, max_positions, device=self.device)
         self.scale = 1.0 / math.sqrt(c.head_dim)
         if ops is None:
@@ -79,8 +75,7 @@ class LlamaEngine:
             and isinstance(weights, LlamaWeights) and os.environ.get("ATLAS_FUSED_NORM", "1") != "0"
         )
         self._folded = self._fold_norms() if self.fused_norm else None
-        if hasattr(ops, "reserve_attention_workspace"):
-            ops.reserve_attention_workspace(64, c.num_heads, c.num_kv_heads, int(max_positions), self.page_size)
+        self._reserve_workspace(int(max_positions))
         self.stats = ForwardStats()
         self._run_lock = threading.RLock()
         self.use_graphs = True
@@ -97,6 +92,47 @@ class LlamaEngine:
         # Graphs captured from now on start with the copy-on-write copy of the plan that rides in
         # the static batch (set by the drafter, whose decode forwards copy tail pages).
         self.cow_in_graph = False
+
+    # ------------------------------------------------------------------
+    # The cache and the ops that touch it (``engine_kv8`` replaces them for the 8-bit cache).
+    def _new_cache(self):
+        c = self.cfg
+        return torch.zeros(
+            (c.num_layers, self.num_pages, 2, c.num_kv_heads, self.page_size, c.head_dim),
+            dtype=self.dtype,
+            device=self.device,
+        )
+
+    def _reserve_workspace(self, max_positions: int) -> None:
+        if hasattr(self.ops, "reserve_attention_workspace"):
+            c = self.cfg
+            self.ops.reserve_attention_workspace(64, c.num_heads, c.num_kv_heads, max_positions, self.page_size)
+
+    def _append(self, qkv, li, positions, slots):
+        """Rotate q and k of ``qkv``, write k and v into layer ``li`` of the cache; returns q."""
+        c = self.cfg
+        return self.ops.rope_qkv_append(qkv, self.rope, positions, slots, self.kv[li], c.num_heads, c.num_kv_heads)
+
+    def _append_normed(self, hb, wqkv, ss, li, positions, slots):
+        """QKV product of the residual copy ``hb`` with folded RMSNorm, then ``_append``."""
+        c = self.cfg
+        return self.ops.qkv_rope(hb, wqkv, ss, c.rms_eps, self.rope, positions, slots, self.kv[li], c.num_heads,
+                                 c.num_kv_heads)
+
+    def _attend(self, q, li, desc, causal_start):
+        o = self.ops
+        if causal_start is None or not hasattr(o, "attention_causal"):
+            return o.attention(q, self.kv[li], desc, self.scale)
+        return o.attention_causal(q, self.kv[li], desc, causal_start, self.scale)
+
+    def _copy_plan(self, plan: torch.Tensor) -> None:
+        self.ops.kv_copy_pages(self.kv, plan)
+
+    def _copy_plan_counted(self, plan: torch.Tensor, count: torch.Tensor) -> None:
+        self.ops.kv_copy_pages_counted(self.kv, plan, count)
+
+    def _move(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        self.ops.kv_move_slots(self.kv, src, dst)
 
     # ------------------------------------------------------------------
     def _fold_norms(self):
@@ -162,7 +198,7 @@ class LlamaEngine:
         n = sb.load(**fields, cow_count=ncow if in_graph else 0)
         if ncow and not in_graph:
             # Tail-page copies (src page, dst page, tokens) before the forward appends to the copies.
-            self.ops.kv_copy_pages(self.kv, sb.aux[: 3 * ncow].view(ncow, 3))
+            self._copy_plan(sb.aux[: 3 * ncow].view(ncow, 3))
         if not graphed:
             logits = self.forward(sb.tokens, sb.positions, sb.slots, sb.desc(prefix_pages))
             return logits[sb.real_slice(n)].clone()
@@ -241,7 +277,7 @@ class LlamaEngine:
             plan = sb.aux[: 3 * sb.M].view(sb.M, 3)
 
             def run():
-                self.ops.kv_copy_pages_counted(self.kv, plan, sb.dparams[3:4])
+                self._copy_plan_counted(plan, sb.dparams[3:4])
                 return fn()
             return run
         if topk:
@@ -325,13 +361,8 @@ class LlamaEngine:
         for li, lw in enumerate(self.w.layers):
             x = o.rmsnorm(h, lw.attn_norm, c.rms_eps, self.dtype)
             qkv = o.linear(x, lw.wqkv)
-            q = o.rope_qkv_append(qkv, self.rope, positions, slots, self.kv[li], c.num_heads, c.num_kv_heads)
-            if causal_start is None:
-                a = o.attention(q, self.kv[li], desc, self.scale)
-            else:
-                a = o.attention_causal(q, self.kv[li], desc, causal_start, self.scale) if hasattr(
-                    o, "attention_causal"
-                ) else o.attention(q, self.kv[li], desc, self.scale)
+            q = self._append(qkv, li, positions, slots)
+            a = self._attend(q, li, desc, causal_start)
             h = o.linear_residual(a, lw.wo, h)
             x = o.rmsnorm(h, lw.mlp_norm, c.rms_eps, self.dtype)
             act = o.gate_up_silu(x, lw.wgu)
@@ -340,12 +371,6 @@ class LlamaEngine:
             h = h.index_select(0, logits_rows.long())
         x = o.rmsnorm(h, self.w.final_norm, c.rms_eps, self.dtype)
         return o.lm_head(x, self.w.lm_head)
-
-    def _attend(self, q, li, desc, causal_start):
-        o = self.ops
-        if causal_start is None:
-            return o.attention(q, self.kv[li], desc, self.scale)
-        return o.attention_causal(q, self.kv[li], desc, causal_start, self.scale)
 
     def _forward_fused(self, tokens, positions, slots, desc, logits_rows, causal_start):
         """CUDA forward with RMSNorm folded into the GEMMs (no norm or RoPE kernels)."""
@@ -363,8 +388,7 @@ class LlamaEngine:
         for li in range(l0, l1):
             lw = self.w.layers[li]
             wqkv, wgu = layers[li]
-            q = o.qkv_rope(hb, wqkv, ss, c.rms_eps, self.rope, positions, slots, self.kv[li], c.num_heads,
-                           c.num_kv_heads)
+            q = self._append_normed(hb, wqkv, ss, li, positions, slots)
             a = self._attend(q, li, desc, causal_start)
             o.linear_residual_norm(a, lw.wo, h, hb, ss)
             act = o.gate_up_silu_norm(hb, wgu, ss, c.rms_eps)
@@ -416,11 +440,11 @@ class LlamaEngine:
 
     def copy_pages(self, copies: torch.Tensor) -> None:
         if copies.numel():
-            self.ops.kv_copy_pages(self.kv, copies.to(self.device))
+            self._copy_plan(copies.to(self.device))
 
     def move_slots(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         if src.numel():
-            self.ops.kv_move_slots(self.kv, src.to(self.device), dst.to(self.device))
+            self._move(src.to(self.device), dst.to(self.device))
 
 
 class CapturedForward(NamedTuple):
@@ -643,6 +667,7 @@ class StaticBatch:
         )
         d._dparams = self.dparams  # type: ignore[attr-defined]
         d._splits = self.engine.graph_attention_splits(self.M)  # type: ignore[attr-defined]
+        d._max_keys = int(self.engine.rope.shape[0])  # type: ignore[attr-defined]
         return d
 
 

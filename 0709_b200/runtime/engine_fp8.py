@@ -38,11 +38,8 @@ class Fp8LlamaEngine(LlamaEngine):
             else:
                 qkv = fp8m.fp8_matmul_ref(torch_ops.rmsnorm(h, lw.attn_norm, c.rms_eps, torch.float32),
                                           lw.wqkv).to(self.dtype)
-            q = o.rope_qkv_append(qkv, self.rope, positions, slots, self.kv[li], c.num_heads, c.num_kv_heads)
-            if causal_start is not None and hasattr(o, "attention_causal"):
-                a = o.attention_causal(q, self.kv[li], desc, causal_start, self.scale)
-            else:
-                a = o.attention(q, self.kv[li], desc, self.scale)
+            q = self._append(qkv, li, positions, slots)
+            a = self._attend(q, li, desc, causal_start)
             if cuda:
                 aq, sa = o.quant_fp8(a)
                 o.gemm_fp8(aq, sa, lw.wo, h, o.ext.EPI_RESIDUAL)

@@ -20,7 +20,7 @@ import torch
 
 from ..models.loader import resolve_model
 from ..runtime.drafter import DrafterRuntime
-from ..runtime.engine import LlamaEngine
+from ..runtime.engine_kv8 import KV_CACHES, make_engine
 from ..utils.timeline import write_timeline_json, write_timeline_svg
 from .edge import DistributedAtlasConfig, PagedDistributedAtlasGenerator
 from .prompts import decode, load_tokenizer, parse_token_ids, required_context_length
@@ -65,7 +65,11 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--timeout", type=float, default=600.0)
     p.add_argument("--trust-remote-code", action="store_true", help="Accepted for compatibility; unused.")
     p.add_argument("--seed", type=int, default=0, help="Seed for random-init presets.")
+    p.add_argument("--drafter-kv-cache", choices=KV_CACHES, default="model",
+                   help="Precision of the drafter's KV cache: the model's, or fp8 (half the bytes per token).")
     # Target options when hosted in process.
+    p.add_argument("--target-kv-cache", choices=KV_CACHES, default="model",
+                   help="Precision of the target's KV cache when it is hosted in process.")
     p.add_argument("--path-score-weights", default=None)
     p.add_argument("--fallback-threshold", type=float, default=None)
     p.add_argument("--first-token-threshold", type=float, default=None)
@@ -87,8 +91,8 @@ def make_target_client(args, ctx: int):
 
     dev = torch.device(args.target_device or (f"cuda:{args.gpu_id}" if torch.cuda.is_available() else "cpu"))
     w = resolve_model(args.target_model, dtype=args.dtype, device=dev, seed=args.seed + 1)
-    eng = LlamaEngine(w, num_pages=2 * math.ceil(ctx / args.page_size) + 64, page_size=args.page_size,
-                      max_positions=ctx + 64)
+    eng = make_engine(w, kv_cache=args.target_kv_cache, num_pages=2 * math.ceil(ctx / args.page_size) + 64,
+                      page_size=args.page_size, max_positions=ctx + 64)
     tv = TargetVerifier(eng, k=args.k, d=args.d, score_weights=parse_score_weights(args.path_score_weights),
                         fallback_threshold=args.fallback_threshold, first_token_threshold=args.first_token_threshold,
                         fallback_ar_tokens=args.fallback_ar_tokens, route_selection_policy=args.route_selection_policy,
@@ -112,7 +116,8 @@ def main(argv=None) -> int:
     dev = torch.device(f"cuda:{args.gpu_id}" if torch.cuda.is_available() else "cpu")
     wd = resolve_model(args.drafter_model, dtype=args.dtype, device=dev, seed=args.seed)
     pages = max(math.ceil(args.max_total_tokens / args.page_size), 2 * math.ceil(ctx / args.page_size) + 64)
-    drafter = DrafterRuntime(LlamaEngine(wd, num_pages=pages, page_size=args.page_size, max_positions=ctx + 64),
+    drafter = DrafterRuntime(make_engine(wd, kv_cache=args.drafter_kv_cache, num_pages=pages, page_size=args.page_size,
+                                         max_positions=ctx + 64),
                              prefill_chunk_size=args.prefill_chunk_size)
     if dev.type == "cuda":
         drafter.warm_graphs(args.k, args.fallback_ar_tokens)

@@ -16,7 +16,7 @@ import math
 import torch
 
 from ..models.loader import resolve_model
-from ..runtime.engine import LlamaEngine
+from ..runtime.engine_kv8 import KV_CACHES, make_engine
 from ..runtime.target import TargetVerifier
 from .rpc import TargetServerApp, serve_target
 
@@ -39,6 +39,9 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--repeat-token-id", type=int, default=42)
     p.add_argument("--page-size", type=int, default=16)
     p.add_argument("--dtype", choices=["float16", "bfloat16", "float32"], default="float16")
+    p.add_argument("--kv-cache", choices=KV_CACHES, default="model",
+                   help="Precision of the KV cache: the model's, or fp8 (e4m3 with a scale per page and head: half the "
+                        "bytes per token).")
     p.add_argument("--device", default="cuda")
     p.add_argument("--seed", type=int, default=0, help="Seed for random-init presets.")
     p.add_argument("--max-new-tokens-capacity", type=int, default=4096,
@@ -71,7 +74,7 @@ def build_backend(args: argparse.Namespace) -> TargetVerifier:
     w = resolve_model(args.model, dtype=args.dtype, device=device, seed=args.seed)
     ctx = int(args.prefix_len) + int(args.max_new_tokens_capacity) + 4 * int(args.k) * int(args.d) + 64
     pages = 2 * math.ceil(ctx / args.page_size) + 64
-    engine = LlamaEngine(w, num_pages=pages, page_size=args.page_size, max_positions=ctx + 64)
+    engine = make_engine(w, kv_cache=args.kv_cache, num_pages=pages, page_size=args.page_size, max_positions=ctx + 64)
     tv = TargetVerifier(
         engine,
         k=args.k,
@@ -100,7 +103,7 @@ def build_multi_session_app(args: argparse.Namespace):
     w = resolve_model(args.model, dtype=args.dtype, device=device, seed=args.seed)
     ctx = int(args.prefix_len) + int(args.max_new_tokens_capacity) + 4 * int(args.k) * int(args.d) + 64
     pages = int(args.sessions) * (2 * math.ceil(ctx / args.page_size) + 64)
-    engine = LlamaEngine(w, num_pages=pages, page_size=args.page_size, max_positions=ctx + 64)
+    engine = make_engine(w, kv_cache=args.kv_cache, num_pages=pages, page_size=args.page_size, max_positions=ctx + 64)
     pool = _native.host().PagePool(engine.num_pages - 1, args.page_size)
 
     def make(sid: str) -> TargetVerifier:
