@@ -25,10 +25,9 @@ __device__ __forceinline__ void decode4(uint32_t w, float* x) {
   x[3] = fb.y;
 }
 
-// One warp folds keys [x0, x1) of row m (kv head h) into its running (ref, l, o); lane t holds
-// dimensions 4 t .. 4 t + 3.  `tail`: the keys' pages are the row's private ones.
-template <bool kTail>
-__device__ __forceinline__ void fold_keys8(const Attn8Params& p, const Attn8Shape& s, int m, int h, int lane,
+// One warp folds keys [x0, x1) of row m (kv head h), in the row's private pages, into its running
+// (ref, l, o); lane t holds dimensions 4 t .. 4 t + 3.
+__device__ __forceinline__ void fold_tail8(const Attn8Params& p, const Attn8Shape& s, int m, int h, int lane,
                                            const float* q, int x0, int x1, int full, int len, float& ref, float& l,
                                            float* o) {
   const int ps = 1 << p.page_shift;
@@ -38,9 +37,7 @@ __device__ __forceinline__ void fold_keys8(const Attn8Params& p, const Attn8Shap
     int64_t ph = -1;
     float ks = 0.f, vs = 0.f;
     if (x < x1 && attn8_visible(p, m, x, full, len, s.mask_base)) {
-      const int j = kTail ? (x >> p.page_shift) - s.n_shared : x >> p.page_shift;
-      const bool in = j >= 0 && j < (kTail ? p.tail_stride : p.n_prefix);
-      const int page = !in ? -1 : kTail ? p.tail_pages[static_cast<int64_t>(m) * p.tail_stride + j] : p.prefix_pages[j];
+      const int page = p.tail_pages[static_cast<int64_t>(m) * p.tail_stride + ((x >> p.page_shift) - s.n_shared)];
       if (page < 0 || page >= p.num_pages) {
         set_error(p.err, kErrBadIndex);
       } else {
@@ -162,7 +159,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
   }
   len_max = __reduce_max_sync(0xffffffffu, len_max);
   full_min = __reduce_min_sync(0xffffffffu, full_min);
-  const int end = min(sh.shared_end, len_max);
+  const int end = attn8_end(p, sh, len_max);
   const int units = (end + 15) >> 4;
   const int per = max((units + p.splits - 1) / p.splits, C::kWarps);
   const int u0 = split * per;
@@ -183,8 +180,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
       w.ks[e] = w.vs[e] = 1.f;
       const int x = ((u0 + warp + (base + lane) * C::kWarps) << 4) + e * 8;
       if (base + lane < mine && x < end && (e == 0 || two)) {
-        const int j = x >> p.page_shift;
-        const int page = j < p.n_prefix ? p.prefix_pages[j] : -1;
+        const int page = p.prefix_pages[x >> p.page_shift];
         if (page < 0 || page >= p.num_pages) {
           set_error(p.err, kErrBadIndex);
         } else {
@@ -268,7 +264,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
   }
 
   bool ok = true;
-  for (int i = 0; i < mine && ok; ++i) {
+  for (int i = 0; i < mine && __all_sync(0xffffffffu, ok); ++i) {
     if (i - window == 32) {
       window += 32;
       cur = nxt;
@@ -276,6 +272,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
     }
     const int stage = i % C::kStages;
     ok = mbar_wait(&bar[stage], (i / C::kStages) & 1, p.err);
+    __syncwarp();  // the matrix instructions need the whole warp together
     const uint8_t* kb = my_ring + stage * C::kUnitBytes;
     const uint8_t* vb = kb + 2048;
     // S: lanes 4 g + t hold keys 8 nt + 2 t, + 1 of rows g and g + 8.
@@ -378,6 +375,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
       }
       pa[mt] = make_uint4(packed[0][0], packed[0][1], packed[1][0], packed[1][1]);
     }
+    __syncwarp();
     // O += P V: lane (g, t) converts dimensions 16 g .. 16 g + 15 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
     uint4 v4[4];
 #pragma unroll
@@ -488,9 +486,11 @@ __global__ void __launch_bounds__(128) attn8_merge_kernel(Attn8Params p) {
   const int len = p.row_len[m], full = min(p.row_full[m], len);
   float o[4] = {0.f, 0.f, 0.f, 0.f}, ref = -INFINITY, l = 0.f;
   if (s.shared_end < len) {
+    const int listed = (s.n_shared + p.tail_stride) << p.page_shift;  // the row's private pages end here
+    if (len > listed && lane == 0) set_error(p.err, kErrBadIndex);
     float q[4];
     load_q4<T>(p, pair, lane, q);
-    fold_keys8<true>(p, s, m, hq / (p.Hq / p.Hkv), lane, q, s.shared_end, len, full, len, ref, l, o);
+    fold_tail8(p, s, m, hq / (p.Hq / p.Hkv), lane, q, s.shared_end, min(len, listed), full, len, ref, l, o);
   }
 
   // A record without keys has sum 0 and no partial row; a NaN sum keeps its weight, so that it shows.

@@ -25,6 +25,13 @@ __device__ __forceinline__ Attn8Shape attn8_shape(const Attn8Params& p) {
   return s;
 }
 
+// End of the shared keys that rows of length up to len_max read, held to the pages that are listed.
+__device__ __forceinline__ int attn8_end(const Attn8Params& p, const Attn8Shape& s, int len_max) {
+  const int end = min(s.shared_end, len_max), listed = p.n_prefix << p.page_shift;
+  if (end > listed) set_error(p.err, kErrBadIndex);
+  return min(end, listed);
+}
+
 // Scales of a page and head as the kernels use them: k scale, log2(v scale), 1 / v scale.  An empty
 // page (scale 0) holds zero codes: any positive scale reads it right.
 __device__ __forceinline__ float4 attn8_scales(const Attn8Params& p, int64_t page_head) {

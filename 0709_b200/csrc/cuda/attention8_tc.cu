@@ -105,13 +105,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float* v) {
 }
 
 // Copy `bytes` (a multiple of 16) from shared to global memory, both 16-byte aligned; the wait returns
-// when this thread's copies have read their source.
+// when the copies of this thread are written (not only read: the merge kernel follows on their heels).
 __device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
                : "memory");
 }
 __device__ __forceinline__ void bulk_store_wait() {
-  asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+  asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 // One lane of a converged warp, the same one every time.
@@ -140,8 +140,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full16 = empty8 + kStages8;
   uint64_t* empty16 = full16 + kStages16;
   uint64_t* s_full = empty16 + kStages16;  // [slot][buffer]
-  uint64_t* p_full = s_full + 4;           // [2], 128 arrivals
-  uint64_t* pv_done = p_full + 2;          // [2]
+  // [slot][buffer], 128 arrivals: a warp may write P(k + 1) while another still works on P(k)
+  uint64_t* p_full = s_full + 4;
+  uint64_t* pv_done = p_full + 4;          // [2]
   uint64_t* q_full = pv_done + 2;          // 512 arrivals
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   int8_t* q_exp = reinterpret_cast<int8_t*>(full8) + 256;  // [256] exponent that scaled each row of Q
@@ -167,7 +168,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[2 * s], 2);
       mbar_init(&s_full[2 * s + 1], 2);
-      mbar_init(&p_full[s], 128);
+      mbar_init(&p_full[2 * s], 128);
+      mbar_init(&p_full[2 * s + 1], 128);
       mbar_init(&pv_done[s], 1);
     }
     mbar_init(q_full, 512);
@@ -210,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int m = row0 / G + lane; m <= (row0 + rows_cta - 1) / G; m += 32) len_max = max(len_max, p.row_len[m]);
     len_max = __reduce_max_sync(0xffffffffu, len_max);
   }
-  const int end = min(sh.shared_end, len_max);
+  const int end = attn8_end(p, sh, len_max);
   const int chunks_all = (end + kChunk - 1) / kChunk;
   const int per = (chunks_all + p.tc_splits - 1) / p.tc_splits;
   const int c0 = static_cast<int>(blockIdx.y) * per;
@@ -250,8 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Window w{0, make_float4(1.f, 0.f, 1.f, 0.f)};
       const int c = first + (lane >> 3), x = (c0 + c) * kChunk + (lane & 7) * 8;
       if (c < chunks && x < end) {
-        const int j = x >> p.page_shift;
-        const int page = j < p.n_prefix ? p.prefix_pages[j] : -1;
+        const int page = p.prefix_pages[x >> p.page_shift];
         if (page < 0 || page >= p.num_pages) {
           set_error(p.err, kErrBadIndex);
         } else {
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (k > 0) {  // P(k - 1) V
           const int j = k - 1, c = ksplit ? 2 * j + slot : j, d = c % kStages16;
-          ok = ok && mbar_wait(&p_full[slot], j & 1, p.err);
+          ok = ok && mbar_wait(&p_full[slot * 2 + (j & 1)], (j >> 1) & 1, p.err);
           tc_fence_after();
           const uint32_t lo = v_lo + d * (kBytes16 >> 4);
           if (leader && ok) {
@@ -400,15 +401,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int n = ksplit ? (chunks + 1 - slot) / 2 : chunks;
     float ref = -INFINITY, sum = 0.f;
     bool ok = true;
-    for (int k = 0; k < n && ok; ++k) {
+    for (int k = 0; k < n && __all_sync(0xffffffffu, ok); ++k) {
       const int c = ksplit ? 2 * k + slot : k;
       const int d = c % kStages16;
       ok = mbar_wait(&s_full[slot * 2 + (k & 1)], (k >> 1) & 1, p.err);
+      __syncwarp();  // TMEM accesses need the whole warp together: after every wait and divergent step
       tc_fence_after();
       const uint32_t tS = tS0 + (k & 1) * 64;
       const int x0 = (c0 + c) * kChunk;
-      const bool partial = x0 + kChunk > sure;
+      // The warp masks as one: rows that see the whole chunk get a mask of ones.
+      const bool partial = __any_sync(0xffffffffu, x0 + kChunk > sure);
       const uint64_t vis = partial ? visible64(p, m, x0, sure, lim, sh.mask_base) : ~0ull;
+      __syncwarp();
       const float4* sc = sc16 + d * 8;
       // Two passes over S, 32 keys at a time (a whole row of S would not fit the registers that 19
       // warps leave): the maximum, then the weights.
@@ -436,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (k > 0) {  // O has to hold P V of every chunk before
           ok = mbar_wait(&pv_done[slot], (k - 1) & 1, p.err) && ok;
+          __syncwarp();
           tc_fence_after();
 #pragma unroll 1
           for (int q4 = 0; q4 < 4; ++q4) {
@@ -448,6 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       const float neg = ref > -INFINITY ? -ref : 0.f;
+      __syncwarp();
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         float s[32], pk[16];
@@ -474,10 +480,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st16(tS + half * 16, pk);  // over keys of the first half, which are read
       }
       tc_fence_before();
-      mbar_arrive(&p_full[slot]);
+      mbar_arrive(&p_full[slot * 2 + (k & 1)]);
     }
     // ---- epilogue
     if (n > 0) ok = mbar_wait(&pv_done[slot], (n - 1) & 1, p.err) && ok;
+    __syncwarp();
     tc_fence_after();
     const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
     const int64_t record = (ksplit ? 2 * blockIdx.y + slot : blockIdx.y) * pairs;

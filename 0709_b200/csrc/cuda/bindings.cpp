@@ -12,6 +12,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <string>
 #include <unordered_map>
 
 #include "attention.h"
@@ -92,7 +93,7 @@ CUtensorMap map_rows(const void* ptr, torch::ScalarType type, int64_t inner, int
   CUresult r = encode_fn()(&m, byte ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : tma_dtype(type), 2, const_cast<void*>(ptr), dims,
                            strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (2d) failed: ", static_cast<int>(r));
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (2d) failed: ", std::to_string(static_cast<int>(r)));
   g_maps.emplace(k, m);
   return m;
 }
@@ -131,7 +132,7 @@ CUtensorMap map_kv(const torch::Tensor& kv) {
   CUresult r = encode_fn()(&m, tma_dtype(kv.scalar_type()), 5, kv.data_ptr(), dims, strides, box, es,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (kv) failed: ", static_cast<int>(r));
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (kv) failed: ", std::to_string(static_cast<int>(r)));
   g_maps.emplace(k, m);
   return m;
 }
@@ -152,7 +153,7 @@ CUtensorMap map_q(const torch::Tensor& q, int64_t G) {
   CUresult r = encode_fn()(&m, tma_dtype(q.scalar_type()), 3, q.data_ptr(), dims, strides, box, es,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (q) failed: ", static_cast<int>(r));
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (q) failed: ", std::to_string(static_cast<int>(r)));
   return m;
 }
 
@@ -324,7 +325,7 @@ std::pair<int, int> fp8_pick_splits(int64_t M, int64_t N, int64_t K, int bn) {
   const int64_t slots = static_cast<int64_t>(num_sms()) * (bn <= 32 ? 2 : 1);  // CTAs resident per SM
   if (tiles * 4 < slots * 3) splits = std::max<int64_t>(1, std::min<int64_t>({kb / 2, slots / tiles, 8}));
   splits = std::max<int64_t>(splits, (kb + atlas::kFp8MaxKbPerCta - 1) / atlas::kFp8MaxKbPerCta);
-  TORCH_CHECK(splits <= 8, "fp8 GEMM: K too long for 8 splits of ", atlas::kFp8MaxKbPerCta, " blocks");
+  TORCH_CHECK(splits <= 8, "fp8 GEMM: K too long for 8 splits of ", std::to_string(atlas::kFp8MaxKbPerCta), " blocks");
   {  // power-of-two cluster sizes (see pick_splits); round up so the scale table still fits
     int64_t p = 1;
     while (p < splits) p *= 2;

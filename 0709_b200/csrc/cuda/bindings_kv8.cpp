@@ -9,12 +9,17 @@
 
 #include <algorithm>
 #include <cmath>
+#include <string>
 
 #include "kv8.h"
 
 namespace {
 
 constexpr double kLog2e = 1.4426950408889634;
+
+// Numbers in messages: streaming one into TORCH_CHECK from this extension ends the process (its copy of
+// the number formatting and torch's do not share their locale).
+std::string str(int64_t n) { return std::to_string(n); }
 
 // A cache data [L, pages, 2, Hkv, ps, 128] e4m3 with scale [L, pages, 2, Hkv], or one of its layers.
 struct Cache8 {
@@ -38,7 +43,7 @@ Cache8 check_cache(const torch::Tensor& data, const torch::Tensor& scale, int64_
                   pages * 2 * Hkv * ps < (int64_t{1} << 31),
               "a layer of the 8-bit cache holds fewer than 2^31 rows of 128 codes");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0, "the 8-bit cache must be 16-byte aligned");
-  TORCH_CHECK(layer >= -1 && layer < L, "layer ", layer, " of a cache of ", L);
+  TORCH_CHECK(layer >= -1 && layer < L, "layer ", str(layer), " of a cache of ", str(L));
   Cache8 c{static_cast<uint8_t*>(data.data_ptr()), scale.data_ptr<float>(), L, pages, Hkv, ps,
            ps == 8 ? 3 : ps == 16 ? 4 : ps == 32 ? 5 : 6};
   if (layer >= 0) {
@@ -52,12 +57,13 @@ Cache8 check_cache(const torch::Tensor& data, const torch::Tensor& scale, int64_
 void check_int(const torch::Tensor& t, const torch::Tensor& like, const char* name, int64_t n = -1) {
   TORCH_CHECK(t.device() == like.device() && t.scalar_type() == torch::kInt32 && t.is_contiguous(), name,
               " must be a contiguous int32 tensor on the cache's device");
-  TORCH_CHECK(n < 0 || t.numel() == n, name, " must hold ", n, " values, not ", t.numel());
+  TORCH_CHECK(n < 0 || t.numel() == n, name, " must hold ", str(n), " values, not ",
+              str(t.numel()));
 }
 
 void check_err(const torch::Tensor& err, const torch::Tensor& like) {
   TORCH_CHECK(err.device() == like.device() && err.scalar_type() == torch::kInt32 && err.numel() >= 1,
-              "the op table belongs to ", err.device(), ", the cache to ", like.device());
+              "the op table belongs to ", err.device().str(), ", the cache to ", like.device().str());
 }
 
 void check_launch(cudaError_t e, const char* what) {
@@ -67,7 +73,7 @@ void check_launch(cudaError_t e, const char* what) {
 torch::Tensor kv8_append(torch::Tensor qkv, torch::Tensor table, torch::Tensor pos, torch::Tensor slots,
                          torch::Tensor data, torch::Tensor scale, int64_t layer, int64_t Hq, bool out_bf16,
                          torch::Tensor err) {
-  TORCH_CHECK(layer >= 0, "layer ", layer);
+  TORCH_CHECK(layer >= 0, "layer ", str(layer));
   const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
   const int64_t Hkv = c.Hkv, M = qkv.size(0);
@@ -133,8 +139,8 @@ void kv8_move_slots(torch::Tensor data, torch::Tensor scale, torch::Tensor src, 
   check_err(err, data);
   check_int(src, data, "source slots");
   check_int(dst, data, "destination slots", src.numel());
-  TORCH_CHECK(src.numel() <= atlas::kKv8MaxMoves, "at most ", atlas::kKv8MaxMoves, " slot moves per call, not ",
-              src.numel());
+  TORCH_CHECK(src.numel() <= atlas::kKv8MaxMoves, "at most ", str(atlas::kKv8MaxMoves), " slot moves per call, not ",
+              str(src.numel()));
   const c10::cuda::CUDAGuard guard(data.device());
   check_launch(atlas::launch_kv8_move_slots(c.data, c.scale, src.data_ptr<int>(), dst.data_ptr<int>(),
                                             static_cast<int>(src.numel()), static_cast<int>(c.layers),
@@ -216,7 +222,7 @@ std::pair<torch::Tensor, int64_t> attention8(
                          c10::optional<torch::Tensor> dparams, int64_t shared_len, int64_t n_shared_pages, int64_t mask_base, torch::Tensor prefix_pages,
                          torch::Tensor row_full, torch::Tensor row_len, torch::Tensor row_mask, torch::Tensor tail_pages,
                          double softmax_scale, int64_t max_keys, torch::Tensor err) {
-  TORCH_CHECK(layer >= 0, "layer ", layer);
+  TORCH_CHECK(layer >= 0, "layer ", str(layer));
   const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
   check_q8(q, data, c, softmax_scale);
@@ -229,6 +235,9 @@ std::pair<torch::Tensor, int64_t> attention8(
               "row_mask must be contiguous int64 [M, words] on the cache's device");
   check_int(tail_pages, data, "tail_pages");
   TORCH_CHECK(tail_pages.dim() == 2 && tail_pages.size(0) == M, "tail_pages must be [M, T]");
+  TORCH_CHECK((prefix_pages.numel() << c.shift) < (1 << 30) &&
+                  ((n_shared_pages + tail_pages.size(1)) << c.shift) < (1 << 30),
+              "the descriptor's page lists must end below position 2^30");
   TORCH_CHECK(shared_len >= 0 && n_shared_pages >= 0 && std::max(shared_len, n_shared_pages << c.shift) < (1 << 30),
               "shared_len and n_shared_pages must be positions below 2^30");
   if (dparams.has_value()) {
@@ -269,7 +278,7 @@ std::pair<torch::Tensor, int64_t> attention8(
 // Row m is at position start + m and sees the keys up to itself, all in prefix_pages.
 torch::Tensor attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tensor scale, int64_t layer,
                                 torch::Tensor prefix_pages, int64_t start, double softmax_scale, torch::Tensor err) {
-  TORCH_CHECK(layer >= 0, "layer ", layer);
+  TORCH_CHECK(layer >= 0, "layer ", str(layer));
   const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
   check_q8(q, data, c, softmax_scale);
@@ -277,8 +286,8 @@ torch::Tensor attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tens
   const int64_t M = q.size(0), ps = c.ps;
   TORCH_CHECK(start >= 0 && start + M < (1 << 30), "positions must be in [0, 2^30)");
   const int64_t n = (start + M + ps - 1) / ps;
-  TORCH_CHECK(n <= prefix_pages.numel(), start + M, " positions need ", n, " pages of ", ps,
-              " slots; the descriptor lists ", prefix_pages.numel());
+  TORCH_CHECK(n <= prefix_pages.numel(), str(start + M), " positions need ", str(n), " pages of ", str(ps),
+              " slots; the descriptor lists ", str(prefix_pages.numel()));
   const c10::cuda::CUDAGuard guard(data.device());
   auto out = torch::empty({M, q.size(1) * 128}, q.options());
   if (M == 0) return out;
