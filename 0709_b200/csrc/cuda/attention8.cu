@@ -35,29 +35,25 @@ __device__ __forceinline__ void fold_tail8(const Attn8Params& p, const Attn8Shap
     // Lane i resolves key t0 + i: its page-head index and scales.
     const int x = t0 + lane;
     int64_t ph = -1;
-    float ks = 0.f, vs = 0.f;
+    float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);
     if (x < x1 && attn8_visible(p, m, x, full, len, s.mask_base)) {
       const int page = p.tail_pages[static_cast<int64_t>(m) * p.tail_stride + ((x >> p.page_shift) - s.n_shared)];
       if (page < 0 || page >= p.num_pages) {
         set_error(p.err, kErrBadIndex);
       } else {
         ph = static_cast<int64_t>(page) * 2 * p.Hkv + h;
-        ks = p.scale[ph];
-        vs = p.scale[ph + p.Hkv];
-        if (!(vs > 0.f)) vs = 1.f;  // an empty page: its codes are zero
+        sc = attn8_scales(p, ph);
       }
     }
     const int cnt = min(32, x1 - t0);
-    for (int j0 = 0; j0 < cnt; j0 += 8) {
-      uint32_t kw[8], vw[8];
-      int64_t pj[8];
-      float kj[8], vj[8];
+    constexpr int kBatch = 4;
+#pragma unroll 1
+    for (int j0 = 0; j0 < cnt; j0 += kBatch) {
+      uint32_t kw[kBatch], vw[kBatch];
+      int64_t pj[kBatch];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int jj = (j0 + u) & 31;
-        pj[u] = __shfl_sync(0xffffffffu, ph, jj);
-        kj[u] = __shfl_sync(0xffffffffu, ks, jj);
-        vj[u] = __shfl_sync(0xffffffffu, vs, jj);
+      for (int u = 0; u < kBatch; ++u) {
+        pj[u] = __shfl_sync(0xffffffffu, ph, j0 + u);
         if (j0 + u >= cnt) pj[u] = -1;
         if (pj[u] >= 0) {
           const uint8_t* kp = p.data + (pj[u] * ps + ((t0 + j0 + u) & (ps - 1))) * kHd + lane * 4;
@@ -66,18 +62,20 @@ __device__ __forceinline__ void fold_tail8(const Attn8Params& p, const Attn8Shap
         }
       }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
+      for (int u = 0; u < kBatch; ++u) {
+        const float4 c = make_float4(__shfl_sync(0xffffffffu, sc.x, j0 + u), __shfl_sync(0xffffffffu, sc.y, j0 + u),
+                                     __shfl_sync(0xffffffffu, sc.z, j0 + u), 0.f);
         if (pj[u] < 0) continue;  // warp-uniform
         float k[4], v[4];
         decode4(kw[u], k);
         decode4(vw[u], v);
         const float dot = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
-        const float sc = dot * kj[u] * p.scale_log2 + log2f(vj[u]);
-        const float nm = fmaxf(ref, sc);
-        const float a = ref > -INFINITY ? exp2f(ref - nm) : 0.f, w = exp2f(sc - nm);
+        const float s2 = fmaf(dot, c.x * p.scale_log2, c.y);
+        const float nm = fmaxf(ref, s2);
+        const float a = ref > -INFINITY ? ex2(ref - nm) : 0.f, w = ex2(s2 - nm);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = o[e] * a + w * v[e];
-        l = l * a + w / vj[u];
+        l = fmaf(w, c.z, l * a);
         ref = nm;
       }
     }
@@ -271,7 +269,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
       nxt = load_window(window + 32);
     }
     const int stage = i % C::kStages;
-    ok = mbar_wait(&bar[stage], (i / C::kStages) & 1, p.err);
+    ok = wait8(&bar[stage], (i / C::kStages) & 1, p.err);
     __syncwarp();  // the matrix instructions need the whole warp together
     const uint8_t* kb = my_ring + stage * C::kUnitBytes;
     const uint8_t* vb = kb + 2048;

@@ -93,4 +93,14 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// mbar_wait as a short loop: the passes here run several roles side by side and are sensitive to the size
+// of their code.
+__device__ __forceinline__ bool wait8(uint64_t* bar, uint32_t parity, int* err) {
+#pragma unroll 1
+  for (uint32_t i = 0; i < kSpinLimit; ++i)
+    if (mbar_try_wait(bar, parity)) return true;
+  set_error(err, kErrWaitTimeout);
+  return false;
+}
+
 }  // namespace atlas

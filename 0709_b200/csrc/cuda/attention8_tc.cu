@@ -184,25 +184,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   pdl_trigger();  // after this CTA's TMEM allocation
 
-  // Q: warps 0-15 bring a sixteenth of the rows each, a row per load of the whole warp (a thread per row
-  // would touch 32 lines with every load), all loads in flight before anything else is read.
-  constexpr int kQRows = ksplit ? 8 : 16;
-  uint2 qraw[kQRows];
-  if (warp < 16) {
-    const int first = warp * kQRows;
-    int qm = (row0 + first) / G, qg = (row0 + first) - qm * G;
-    const uint2* src = reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + lane * 4);
-#pragma unroll
-    for (int i = 0; i < kQRows; ++i) {
-      qraw[i] = make_uint2(0, 0);
-      if (first + i < rows_cta) qraw[i] = src[(static_cast<int64_t>(qm) * p.Hq + h * G + qg) * (kHd / 4)];
-      if (++qg == G) {
-        qg = 0;
-        ++qm;
-      }
-    }
-  }
-
   // This split's chunks: up to the last key that any row of the CTA may see.
   const Attn8Shape sh = attn8_shape(p);
   int len_max = 0;
@@ -220,20 +201,39 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int ps = 1 << p.page_shift;
 
   if (warp < 16) {
-    // Each row scaled by a power of two so that its largest element is in [1, 2), as fp16, swizzled.
+    // Q: a sixteenth of the rows per warp, a row per load of the whole warp (a thread per row would touch
+    // 32 lines with every load), each row scaled by a power of two so that its largest element is in
+    // [1, 2), as fp16, swizzled.  Four rows at a time: code that runs once costs more to fetch than to
+    // run, and all sixteen rows unrolled took longer.
+    constexpr int kQRows = ksplit ? 8 : 16;
+    int row = warp * kQRows;
+    int qm = (row0 + row) / G, qg = (row0 + row) - qm * G;
+    const uint2* src = reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + h * G * kHd + lane * 4);
+#pragma unroll 1
+    for (int i0 = 0; i0 < kQRows; i0 += 4) {
+      uint2 w[4];
 #pragma unroll
-    for (int i = 0; i < kQRows; ++i) {
-      const T* e = reinterpret_cast<const T*>(&qraw[i]);
-      const float q[4] = {to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
-      const float am = fmaxf(max3(fabsf(q[0]), fabsf(q[1]), fabsf(q[2])), fabsf(q[3]));
-      const int e2 = row_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(am)));
-      const float down = __int_as_float((127 - e2) << 23);
-      const int row = warp * kQRows + i;
-      uint8_t* qs = row < 128 ? q_s : q1_s;
-      *reinterpret_cast<uint2*>(qs + (lane >> 4) * (kBytesQ / 2) + (lane & 1) * 8 +
-                                sw128_offset(row & 127, (lane & 15) >> 1)) =
-          make_uint2(pack_half2(q[0] * down, q[1] * down), pack_half2(q[2] * down, q[3] * down));
-      if (lane == 0) q_exp[row] = static_cast<int8_t>(e2);
+      for (int i = 0; i < 4; ++i) {
+        w[i] = make_uint2(0, 0);
+        if (row + i < rows_cta) w[i] = src[(static_cast<int64_t>(qm) * p.Hq + qg) * (kHd / 4)];
+        if (++qg == G) {
+          qg = 0;
+          ++qm;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i, ++row) {
+        const T* e = reinterpret_cast<const T*>(&w[i]);
+        const float q[4] = {to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
+        const float am = fmaxf(max3(fabsf(q[0]), fabsf(q[1]), fabsf(q[2])), fabsf(q[3]));
+        const int e2 = row_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(am)));
+        const float down = __int_as_float((127 - e2) << 23);
+        uint8_t* qs = row < 128 ? q_s : q1_s;
+        *reinterpret_cast<uint2*>(qs + (lane >> 4) * (kBytesQ / 2) + (lane & 1) * 8 +
+                                  sw128_offset(row & 127, (lane & 15) >> 1)) =
+            make_uint2(pack_half2(q[0] * down, q[1] * down), pack_half2(q[2] * down, q[3] * down));
+        if (lane == 0) q_exp[row] = static_cast<int8_t>(e2);
+      }
     }
     fence_proxy_async_smem();
     mbar_arrive(q_full);
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       sc.y = __shfl_sync(0xffffffffu, cur.sc.y, from);
       sc.z = __shfl_sync(0xffffffffu, cur.sc.z, from);
       sc.w = 0.f;
-      bool ok = c < kStages8 || mbar_wait(&empty8[s], ((c / kStages8) - 1) & 1, p.err);
+      bool ok = c < kStages8 || wait8(&empty8[s], ((c / kStages8) - 1) & 1, p.err);
       if (!__all_sync(0xffffffffu, ok)) break;
       if (lane < 8) sc8[s * 8 + lane] = sc;
       __syncwarp();
@@ -298,8 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int c = (warp - 8) >> 2; c < chunks && ok; c += 2) {
       const int s = c % kStages8, d = c % kStages16;
-      ok = mbar_wait(&full8[s], (c / kStages8) & 1, p.err);
-      if (ok && c >= kStages16) ok = mbar_wait(&empty16[d], ((c / kStages16) - 1) & 1, p.err);
+      ok = wait8(&full8[s], (c / kStages8) & 1, p.err);
+      if (ok && c >= kStages16) ok = wait8(&empty16[d], ((c / kStages16) - 1) & 1, p.err);
       if (!ok) break;
       if ((tid & 127) < 8) sc16[d * 8 + (tid & 127)] = sc8[s * 8 + (tid & 127)];
       const uint8_t* src = ring8 + s * kBytes8;
@@ -343,12 +343,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t v_lo = ((smem_u32(ring16) + 2 * kHalf16) >> 4) | (kHalf16 >> 4) << 16;
       const uint32_t tS0 = tmem + slot * 128, tO = tmem + kColO + slot * 128;
       const bool leader = elect_one();
-      bool ok = mbar_wait(q_full, 0, p.err);
+      bool ok = wait8(q_full, 0, p.err);
       for (int k = 0; k <= n && ok; ++k) {
         if (k < n) {  // S(k); its buffer holds P(k - 2) until that P V is done
           const int c = ksplit ? 2 * k + slot : k, d = c % kStages16;
-          if (k >= 2) ok = mbar_wait(&pv_done[slot], k & 1, p.err);
-          ok = ok && mbar_wait(&full16[d], (c / kStages16) & 1, p.err);
+          if (k >= 2) ok = wait8(&pv_done[slot], k & 1, p.err);
+          ok = ok && wait8(&full16[d], (c / kStages16) & 1, p.err);
           tc_fence_after();
           const uint32_t lo = k_lo + d * (kBytes16 >> 4);
           if (leader && ok) {
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (k > 0) {  // P(k - 1) V
           const int j = k - 1, c = ksplit ? 2 * j + slot : j, d = c % kStages16;
-          ok = ok && mbar_wait(&p_full[slot * 2 + (j & 1)], (j >> 1) & 1, p.err);
+          ok = ok && wait8(&p_full[slot * 2 + (j & 1)], (j >> 1) & 1, p.err);
           tc_fence_after();
           const uint32_t lo = v_lo + d * (kBytes16 >> 4);
           if (leader && ok) {
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       full = p.causal_start >= 0 ? len : min(p.row_full[m], len);
     }
     const int lim = min(len, end), sure = min(full, end);  // keys below `sure` are visible
-    mbar_wait(q_full, 0, p.err);
+    wait8(q_full, 0, p.err);
     const int e2 = q_exp[r];
     const float fac = p.scale_log2 * __int_as_float((127 + e2) << 23);
 
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int k = 0; k < n && __all_sync(0xffffffffu, ok); ++k) {
       const int c = ksplit ? 2 * k + slot : k;
       const int d = c % kStages16;
-      ok = mbar_wait(&s_full[slot * 2 + (k & 1)], (k >> 1) & 1, p.err);
+      ok = wait8(&s_full[slot * 2 + (k & 1)], (k >> 1) & 1, p.err);
       __syncwarp();  // TMEM accesses need the whole warp together: after every wait and divergent step
       tc_fence_after();
       const uint32_t tS = tS0 + (k & 1) * 64;
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Two passes over S, 32 keys at a time (a whole row of S would not fit the registers that 19
       // warps leave): the maximum, then the weights.
       float top = -INFINITY;
-#pragma unroll
+#pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         float s[32];
         tmem_ld32(tS + half * 32, s);
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           sum *= a;
         }
         if (k > 0) {  // O has to hold P V of every chunk before
-          ok = mbar_wait(&pv_done[slot], (k - 1) & 1, p.err) && ok;
+          ok = wait8(&pv_done[slot], (k - 1) & 1, p.err) && ok;
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float neg = ref > -INFINITY ? -ref : 0.f;
       __syncwarp();
-#pragma unroll
+#pragma unroll 1
       for (int half = 0; half < 2; ++half) {
         float s[32], pk[16];
         tmem_ld32(tS + half * 32, s);
@@ -483,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive(&p_full[slot * 2 + (k & 1)]);
     }
     // ---- epilogue
-    if (n > 0) ok = mbar_wait(&pv_done[slot], (n - 1) & 1, p.err) && ok;
+    if (n > 0) ok = wait8(&pv_done[slot], (n - 1) & 1, p.err) && ok;
     __syncwarp();
     tc_fence_after();
     const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
