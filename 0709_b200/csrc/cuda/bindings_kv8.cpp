@@ -169,9 +169,12 @@ torch::Tensor kv8_read_pages(torch::Tensor data, torch::Tensor scale, int64_t la
 }
 
 // The split pass's launch shape for `rows` query rows of a kv head (query rows times group).  Up to 32
-// rows go through the register tensor-core pass in tiles of 16 or 32; more through the tcgen05 pass,
-// whose CTA holds 128 rows over alternate chunks of keys or, above 128, 256 rows.  The splits fill the
-// CTA slots (two per SM for the small tile) with at least 128 keys each.
+// rows go through the register tensor-core pass in tiles of 16 or 32 rows; more through the tcgen05
+// pass, whose CTA holds 128 rows over alternate chunks of keys or, above 128, 256 rows (8 kv heads, us:
+// 32 rows on 16K keys 24.8 against 28.5, 48 rows 34.6 against 29.9).  The splits fill the CTA slots
+// (two per SM for the small tile) with at least 128 keys each up to eight splits and 256 beyond (36
+// rows on 2051 keys: 17 splits 16.8 us, 9 splits 15.1 us; 48 rows on 1000 keys: 8 splits 10.9 us, 4
+// splits 12.4 us).
 void pick_shape8(atlas::Attn8Params& p, int64_t rows, int64_t keys, int sms) {
   p.row_tile = rows <= 16 ? 16 : rows <= 32 ? 32 : 0;
   p.tc_ksplit = rows <= 128 ? 1 : 0;
@@ -179,7 +182,8 @@ void pick_shape8(atlas::Attn8Params& p, int64_t rows, int64_t keys, int sms) {
   const int64_t slots = static_cast<int64_t>(sms) * (p.row_tile == 16 ? 2 : 1);
   const int64_t ctas = p.Hkv * ((rows + tile - 1) / tile);
   const int64_t most = p.row_tile == 0 && p.tc_ksplit ? 32 : 64;  // records
-  const int64_t n = std::max<int64_t>(1, std::min<int64_t>({most, slots / ctas, (keys + 127) / 128}));
+  const int64_t useful = std::max<int64_t>((keys + 255) / 256, std::min<int64_t>(8, (keys + 127) / 128));
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>({most, slots / ctas, useful}));
   p.tc_splits = static_cast<int>(n);
   p.splits = static_cast<int>(most == 32 ? 2 * n : n);
 }
