@@ -5,6 +5,7 @@
 #include "bindings_kv8.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
@@ -66,6 +67,11 @@ void check_err(const torch::Tensor& err, const torch::Tensor& like) {
               "the op table belongs to ", err.device().str(), ", the cache to ", like.device().str());
 }
 
+// An uninitialized tensor on `like`'s device, without the dispatcher's round (small calls are host-bound).
+torch::Tensor fresh(at::IntArrayRef size, torch::ScalarType type, const torch::Tensor& like) {
+  return at::detail::empty_cuda(size, type, like.device(), c10::nullopt);
+}
+
 void check_launch(cudaError_t e, const char* what) {
   TORCH_CHECK(e == cudaSuccess, what, ": ", cudaGetErrorString(e));
 }
@@ -92,7 +98,7 @@ torch::Tensor kv8_append(torch::Tensor qkv, torch::Tensor table, torch::Tensor p
   TORCH_CHECK(M * (Hq + Hkv) < (int64_t{1} << 31), "kv8 append size");
   const bool bf16 = t == torch::kFloat32 ? out_bf16 : t == torch::kBFloat16;
   const c10::cuda::CUDAGuard guard(data.device());
-  auto q = torch::empty({M, Hq, 128}, qkv.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf));
+  auto q = fresh({M, Hq, 128}, bf16 ? torch::kBFloat16 : torch::kHalf, data);
   atlas::Kv8AppendParams p{};
   p.qkv = qkv.data_ptr();
   p.table = table.data_ptr<float>();
@@ -157,9 +163,9 @@ torch::Tensor kv8_read_pages(torch::Tensor data, torch::Tensor scale, int64_t la
   check_int(pages, data, "pages");
   const int64_t n = pages.numel();
   const c10::cuda::CUDAGuard guard(data.device());
-  const auto opt = data.options().dtype(bf16 ? torch::kBFloat16 : torch::kHalf);
-  auto out = layer < 0 ? torch::empty({c.layers, n, 2, c.Hkv, c.ps, 128}, opt)
-                       : torch::empty({n, 2, c.Hkv, c.ps, 128}, opt);
+  const auto type = bf16 ? torch::kBFloat16 : torch::kHalf;
+  auto out = layer < 0 ? fresh({c.layers, n, 2, c.Hkv, c.ps, 128}, type, data)
+                       : fresh({n, 2, c.Hkv, c.ps, 128}, type, data);
   check_launch(atlas::launch_kv8_read_pages(c.data, c.scale, pages.data_ptr<int>(), out.data_ptr(),
                                             static_cast<int>(n), static_cast<int>(c.layers),
                                             static_cast<int>(c.pages), static_cast<int>(c.Hkv), c.shift, bf16,
@@ -249,7 +255,7 @@ std::pair<torch::Tensor, int64_t> attention8(
     TORCH_CHECK(dparams->numel() >= 3, "the descriptor's device scalars are shared_len, n_shared_pages, mask_base");
   }
   const c10::cuda::CUDAGuard guard(data.device());
-  auto out = torch::empty({M, Hq * 128}, q.options());
+  auto out = fresh({M, Hq * 128}, q.scalar_type(), data);
   if (M == 0) return {out, 0};
   atlas::Attn8Params p = params8(q, c, out, prefix_pages, softmax_scale, err);
   p.dparams = dparams.has_value() ? dparams->data_ptr<int>() : nullptr;
@@ -271,7 +277,7 @@ std::pair<torch::Tensor, int64_t> attention8(
   }
   torch::Tensor parts;
   if (p.splits > 0) {
-    parts = torch::empty({p.splits * M * Hq * 130}, q.options().dtype(torch::kFloat32));
+    parts = fresh({p.splits * M * Hq * 130}, torch::kFloat32, data);
     p.part_o = parts.data_ptr<float>();
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<int64_t>(p.splits) * M * Hq * 128);
   }
@@ -293,7 +299,7 @@ torch::Tensor attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tens
   TORCH_CHECK(n <= prefix_pages.numel(), str(start + M), " positions need ", str(n), " pages of ", str(ps),
               " slots; the descriptor lists ", str(prefix_pages.numel()));
   const c10::cuda::CUDAGuard guard(data.device());
-  auto out = torch::empty({M, q.size(1) * 128}, q.options());
+  auto out = fresh({M, q.size(1) * 128}, q.scalar_type(), data);
   if (M == 0) return out;
   atlas::Attn8Params p = params8(q, c, out, prefix_pages, softmax_scale, err);
   p.causal_start = static_cast<int>(start);
