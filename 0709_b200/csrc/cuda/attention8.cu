@@ -146,6 +146,18 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
   __syncwarp();
   pdl_wait();
   pdl_trigger();
+  // The tile's Q rows, a row per load of a warp, on their way before anything waits for memory.
+  constexpr int kQRows = C::kRows / C::kWarps;
+  uint2 qraw[kQRows];
+#pragma unroll
+  for (int i = 0; i < kQRows; ++i) {
+    const int grow = tile0 + warp + i * C::kWarps;
+    const int m = grow / G;
+    qraw[i] = make_uint2(0, 0);
+    if (grow < rows_total)
+      qraw[i] = *reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) +
+                                                (static_cast<int64_t>(m) * p.Hq + h * G + grow - m * G) * kHd + lane * 4);
+  }
   const Attn8Shape sh = attn8_shape(p);
 
   // The tile's limits: last visible key of any row, first key that some row may not see.
@@ -225,14 +237,14 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
   // Q rows as fp16 A fragments, each row scaled by a power of two so that its largest element is in
   // [1, 2): bf16 rows of any size fit.  Dimensions 16 (2 t + s) + 4 i .. + 3 of a row belong to k-step
   // 4 s + i of the lanes t: the bytes of the K word that these lanes convert.
-  for (int r = warp; r < C::kRows; r += C::kWarps) {
-    float q[4] = {0.f, 0.f, 0.f, 0.f};
-    const int grow = tile0 + r;
-    if (grow < rows_total)
-      load_q4<T>(p, static_cast<int64_t>(grow / G) * p.Hq + h * G + grow % G, lane, q);
+#pragma unroll
+  for (int i = 0; i < kQRows; ++i) {
+    const int r = warp + i * C::kWarps;
+    const T* e = reinterpret_cast<const T*>(&qraw[i]);
+    const float q[4] = {to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
     uint32_t ab = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ab = max(ab, __float_as_uint(q[e]) & 0x7fffffffu);
+    for (int k = 0; k < 4; ++k) ab = max(ab, __float_as_uint(q[k]) & 0x7fffffffu);
     ab = __reduce_max_sync(0xffffffffu, ab);
     const int e2 = row_exponent(ab);
     const float down = __int_as_float((127 - e2) << 23);
@@ -425,10 +437,11 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
       }
     }
   __syncthreads();
+#pragma unroll
   for (int it = tid; it < C::kRows * 32; it += 256) {
     const int r = it >> 5, f = it & 31;  // one warp per row
     const int grow = tile0 + r;
-    if (grow >= rows_total) continue;
+    if (grow >= rows_total) break;  // whole warps, rows in order
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < C::kWarps) ml = ml_s[lane * C::kRows + r];
     if (ml.y == 0.f) ml.x = -INFINITY;
