@@ -494,9 +494,10 @@ __global__ void __launch_bounds__(128) attn8_merge_kernel(Attn8Params p) {
     if (j < S) ov[j] = __ldcg(reinterpret_cast<const float4*>(po + j * pairs * kHd));
 
   const Attn8Shape s = attn8_shape(p);
-  const int len = p.row_len[m], full = min(p.row_full[m], len);
   float o[4] = {0.f, 0.f, 0.f, 0.f}, ref = -INFINITY, l = 0.f;
+  const int len = p.causal_start >= 0 ? 0 : p.row_len[m];  // a causal chunk has no private pages
   if (s.shared_end < len) {
+    const int full = min(p.row_full[m], len);
     const int listed = (s.n_shared + p.tail_stride) << p.page_shift;  // the row's private pages end here
     if (len > listed && lane == 0) set_error(p.err, kErrBadIndex);
     float q[4];
@@ -565,6 +566,7 @@ static cudaError_t launch_typed8(const CUtensorMap& map, const Attn8Params& p, c
 
 cudaError_t launch_attention8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
   if (p.M == 0) return cudaSuccess;
+  if (p.direct) return launch_attention8_tc(map, p, st);
   return p.bf16 ? launch_typed8<__nv_bfloat16>(map, p, st) : launch_typed8<__half>(map, p, st);
 }
 

@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
     const int64_t record = (ksplit ? 2 * blockIdx.y + slot : blockIdx.y) * pairs;
-    const bool direct = p.causal_start >= 0;
+    const bool direct = p.direct != 0;
     if (live && !direct) p.part_ml[record + pair] = make_float2(ref, sum);
     // O by way of shared memory (the chunks' space, once both slots are done with it): a thread lays its
     // row down and copies it out as one bulk transfer.  Rows are padded by 16 bytes against bank conflicts.

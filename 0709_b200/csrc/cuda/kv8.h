@@ -62,12 +62,14 @@ struct Attn8Params {
   int row_tile;      // query rows of a kv head per CTA of the split pass: 16, 32, or 0 for the tcgen05 pass
   int tc_splits;     // tcgen05 pass: key splits (grid), each two records when tc_ksplit
   int tc_ksplit;     // both slots of a CTA hold the same 128 rows and take alternate chunks
-  int causal_start;  // >= 0: row m is at position causal_start + m and sees the keys up to itself; writes `out`
+  int causal_start;  // >= 0: row m is at position causal_start + m and sees the keys up to itself
+  int direct;        // tcgen05 pass: one split, writes `out` itself
   float scale_log2;  // softmax scale * log2(e)
 };
 // map: the layer as rows of 128 bytes, box (128, min(page size, 16)), 128B swizzle.
 cudaError_t launch_attention8(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st);
 
+// The tcgen05 pass alone: all there is to a direct call.
 cudaError_t launch_attention8_tc(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st);
 
 }  // namespace atlas

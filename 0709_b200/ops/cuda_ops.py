@@ -339,9 +339,9 @@ class CudaOps:
         """Attention of a prefill chunk at positions ``causal_start ..`` whose own keys are in the 8-bit cache
         already; the descriptor gives the page list."""
         scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-        out = self.ext.attention8_causal(q, kv_layer.cache.data, kv_layer.cache.scale, kv_layer.index,
-                                         desc.prefix_pages, int(causal_start), scale, self.err)
-        counters.launches(1)
+        out, launches = self.ext.attention8_causal(q, kv_layer.cache.data, kv_layer.cache.scale, kv_layer.index,
+                                                   desc.prefix_pages, int(causal_start), scale, self.err)
+        counters.launches(launches)
         return out
 
     def kv8_copy_pages(self, cache, copies: torch.Tensor) -> None:

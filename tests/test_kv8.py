@@ -428,7 +428,8 @@ def test_attention_scale_and_sharp_scores(device):
 @pytest.mark.parametrize("device", IMPLS)
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("ps,hq,hkv,start,rows", [(16, 4, 2, 0, 1), (16, 8, 2, 0, 45), (8, 8, 8, 77, 30),
-                                                  (32, 16, 2, 300, 129), (64, 4, 4, 13, 64)])
+                                                  (32, 16, 2, 300, 129), (64, 4, 4, 13, 64),
+                                                  (16, 8, 2, 1500, 3), (16, 4, 2, 900, 70)])
 def test_attention_causal(device, dtype, ps, hq, hkv, start, rows):
     ops = impl(device)
     pages = 4 + -(-(start + rows) // ps)
