@@ -2,13 +2,13 @@
 //
 // One CTA holds two tiles ("slots") of 128 query rows of one kv head: two different row tiles over
 // the same keys, or -- when one tile holds all rows -- the same rows over alternate 64-key chunks,
-// each slot then being a split of its own.  19 warps:
+// each slot then being a split of its own.  Warps:
 //   0-7   softmax, one thread per query row (0-3 slot 0, 4-7 slot 1);
-//   8-15  converters: e4m3 codes of a chunk -> fp16 operand tiles in the 128B-swizzled layout (two
-//         groups of four warps, alternate chunks);
-//   16    TMA producer: the chunk's pages (K and V codes) and their scales;
-//   17-18 MMA issuers, one per slot (one for both spent its time in turn on waits and issue: 2450
-//         cycles per pair of S and P V tiles whose products take 1280).
+//   8-    converters: e4m3 codes of a chunk -> fp16 operand tiles in the 128B-swizzled layout (four
+//         warps, or two groups of four on alternate chunks);
+//   then  the TMA producer (the chunk's pages, K and V codes, and their scales) and two MMA issuers, one
+//         per slot (one for both spent its time in turn on waits and issue: 2450 cycles per pair of S and
+//         P V tiles whose products take 1280).
 // S is double-buffered in TMEM, so that a slot's next scores are ready when its softmax is; P (fp16)
 // replaces its S in place and is the A operand of O += P V.  Q is read from shared memory (TMEM has no
 // room left).  Per 64-key chunk the shared memory carries the codes (16 KB written, 16 KB read), the
@@ -29,7 +29,13 @@ constexpr int kBytes16 = 4 * kHalf16;          // K halves | V halves
 constexpr int kBytesQ = 128 * kHd * 2;         // two halves of 128 rows x 128 B
 static_assert(256 * (kHd * 4 + 16) <= kStages8 * kBytes8 + 4 * kBytes16, "the output rows reuse the chunks' space");
 static_assert(kBytesQ == kBytes16, "slot 1's own Q takes the place of the fourth converted chunk");
-constexpr int kThreads = 608;
+// Converter groups of four warps: with split keys a chunk feeds one slot only and two groups keep up.
+template <bool kSplitKeys>
+struct Roles {
+  static constexpr int kConvGroups = kSplitKeys ? 2 : 1;
+  static constexpr int kProducer = 8 + 4 * kConvGroups;
+  static constexpr int kThreads = (kProducer + 3) * 32;
+};
 constexpr int kSmem = 1024 + kStages8 * kBytes8 + 4 * kBytes16 + kBytesQ + (kStages8 + 4) * 128 + 256 + 256;
 constexpr uint32_t kColO = 256;
 constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
@@ -122,9 +128,10 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 template <typename T, bool kSplitKeys>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
     attn8_tc_kernel(const __grid_constant__ CUtensorMap map, Attn8Params p) {
   constexpr bool ksplit = kSplitKeys;
+  using R = Roles<kSplitKeys>;
   constexpr int kStages16 = kSplitKeys ? 4 : 3;  // converted chunks
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -143,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // [slot][buffer], 128 arrivals: a warp may write P(k + 1) while another still works on P(k)
   uint64_t* p_full = s_full + 4;
   uint64_t* pv_done = p_full + 4;          // [2]
-  uint64_t* q_full = pv_done + 2;          // 512 arrivals
+  uint64_t* q_full = pv_done + 2;          // every staging thread
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   int8_t* q_exp = reinterpret_cast<int8_t*>(full8) + 256;  // [256] exponent that scaled each row of Q
 
@@ -172,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&p_full[2 * s + 1], 128);
       mbar_init(&pv_done[s], 1);
     }
-    mbar_init(q_full, 512);
+    mbar_init(q_full, R::kProducer * 32);
     fence_barrier_init();
     tma_prefetch_desc(&map);
   }
@@ -200,12 +207,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int chunks = max(0, min(chunks_all, c0 + per) - c0);
   const int ps = 1 << p.page_shift;
 
-  if (warp < 16) {
-    // Q: a sixteenth of the rows per warp, a row per load of the whole warp (a thread per row would touch
+  if (warp < R::kProducer) {
+    // Q: an equal share of the rows per warp, a row per load of the whole warp (a thread per row would touch
     // 32 lines with every load), each row scaled by a power of two so that its largest element is in
     // [1, 2), as fp16, swizzled.  Four rows at a time: code that runs once costs more to fetch than to
     // run, and all sixteen rows unrolled took longer.
-    constexpr int kQRows = ksplit ? 8 : 16;
+    constexpr int kQRows = ksplit ? 8 : 24;  // rows past the tile are not kept
     int row = warp * kQRows;
     int qm = (row0 + row) / G, qg = (row0 + row) - qm * G;
     const uint2* src = reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + h * G * kHd + lane * 4);
@@ -229,17 +236,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int e2 = row_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(am)));
         const float down = __int_as_float((127 - e2) << 23);
         uint8_t* qs = row < 128 ? q_s : q1_s;
-        *reinterpret_cast<uint2*>(qs + (lane >> 4) * (kBytesQ / 2) + (lane & 1) * 8 +
-                                  sw128_offset(row & 127, (lane & 15) >> 1)) =
-            make_uint2(pack_half2(q[0] * down, q[1] * down), pack_half2(q[2] * down, q[3] * down));
-        if (lane == 0) q_exp[row] = static_cast<int8_t>(e2);
+        if (row < 256) {
+          *reinterpret_cast<uint2*>(qs + (lane >> 4) * (kBytesQ / 2) + (lane & 1) * 8 +
+                                    sw128_offset(row & 127, (lane & 15) >> 1)) =
+              make_uint2(pack_half2(q[0] * down, q[1] * down), pack_half2(q[2] * down, q[3] * down));
+          if (lane == 0) q_exp[row] = static_cast<int8_t>(e2);
+        }
       }
     }
     fence_proxy_async_smem();
     mbar_arrive(q_full);
   }
 
-  if (warp == 16) {
+  if (warp == R::kProducer) {
     // ---- producer.  Lane l holds page and scales of 8 keys, l & 7, of chunk l >> 3 of a window of
     // four; the next window is loaded while this one is issued (page and scale are two dependent
     // trips to memory: taken chunk by chunk they bound the pass at 2 TB/s).
@@ -289,14 +298,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_2d(dst + kBytes8 / 2, &map, &full8[s], 0, y + p.Hkv * ps);
       }
     }
-  } else if (warp >= 8 && warp < 16) {
+  } else if (warp >= 8 && warp < R::kProducer) {
     // ---- converters: one 16-byte piece of codes (16 dimensions of a key) per thread and step
     // Pieces p and p + 4 of a row would meet the same banks (its two 64-dimension halves): the upper
     // pieces take the neighbouring row.
     const int piece = tid & 7, upper = piece >> 2;
     const int row = ((tid & 127) >> 3) ^ upper;  // rows row, row + 16, ..
     bool ok = true;
-    for (int c = (warp - 8) >> 2; c < chunks && ok; c += 2) {
+    for (int c = (warp - 8) >> 2; c < chunks && ok; c += R::kConvGroups) {
       const int s = c % kStages8, d = c % kStages16;
       ok = wait8(&full8[s], (c / kStages8) & 1, p.err);
       if (ok && c >= kStages16) ok = wait8(&empty16[d], ((c / kStages16) - 1) & 1, p.err);
@@ -328,11 +337,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_proxy_async_smem();
       mbar_arrive(&full16[d]);
     }
-  } else if (warp >= 17) {
+  } else if (warp > R::kProducer) {
     // ---- MMA issuer of a slot.  The whole warp walks the loop and one elected lane issues: addresses
     // and descriptors then live in uniform registers (a single thread that builds each descriptor took
     // about 700 cycles for the eight instructions of an S tile, more than the products themselves).
-    const int slot = warp - 17;
+    const int slot = warp - R::kProducer - 1;
     const int n = ksplit ? (chunks + 1 - slot) / 2 : chunks;
     if (n > 0) {
       constexpr uint32_t idesc_s = umma_idesc_f16(128, kChunk, false, false, false);
@@ -414,21 +423,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t vis = partial ? visible64(p, m, x0, sure, lim, sh.mask_base) : ~0ull;
       __syncwarp();
       const float4* sc = sc16 + d * 8;
-      // Two passes over S, 32 keys at a time (a whole row of S would not fit the registers that 19
-      // warps leave): the maximum, then the weights.
+      // S 32 keys at a time.  With eight converter warps a row of S does not fit the registers and is read
+      // twice, for the maximum and for the weights; with four it stays.
+      constexpr int kKept = ksplit ? 1 : 2;
+      float s[kKept][32];
       float top = -INFINITY;
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        float s[32];
-        tmem_ld32(tS + half * 32, s);
-        if (partial) hide(s, vis >> (half * 32));
+      auto load_half = [&](int half, float* v) {
+        tmem_ld32(tS + half * 32, v);
+        if (partial) hide(v, vis >> (half * 32));
+      };
+      auto half_top = [&](int half, const float* v) {
 #pragma unroll
-        for (int gk = 0; gk < 4; ++gk) {
+        for (int gk = 0; gk < 4; ++gk, v += 8) {
           const float4 w = sc[half * 4 + gk];
-          const float* v = s + gk * 8;
           const float mx = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
           top = fmaxf(top, fmaf(mx, fac * w.x, w.y));
         }
+      };
+      if constexpr (ksplit) {
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          load_half(half, s[0]);
+          half_top(half, s[0]);
+        }
+      } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) load_half(half, s[half % kKept]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) half_top(half, s[half % kKept]);
       }
       const bool grow_ref = top > ref + kGrow;
       if (__any_sync(0xffffffffu, grow_ref)) {
@@ -454,11 +476,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const float neg = ref > -INFINITY ? -ref : 0.f;
       __syncwarp();
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        float s[32], pk[16];
-        tmem_ld32(tS + half * 32, s);
-        if (partial) hide(s, vis >> (half * 32));
+      auto weigh_half = [&](int half, const float* v) {
+        float pk[16];
 #pragma unroll
         for (int gk = 0; gk < 4; ++gk) {
           const float4 w = sc[half * 4 + gk];
@@ -467,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 8; j += 2) {
             float p0, p1;
-            unpair2(fma2(pair2(s[gk * 8 + j], s[gk * 8 + j + 1]), f, b), p0, p1);
+            unpair2(fma2(pair2(v[gk * 8 + j], v[gk * 8 + j + 1]), f, b), p0, p1);
             p0 = ex2(p0);
             p1 = ex2(p1);
             acc = add2(acc, pair2(p0, p1));
@@ -478,6 +497,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           sum = fmaf(a0 + a1, w.z, sum);
         }
         tmem_st16(tS + half * 16, pk);  // over keys of the first half, which are read
+      };
+      if constexpr (ksplit) {
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          load_half(half, s[0]);
+          weigh_half(half, s[0]);
+        }
+      } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) weigh_half(half, s[half % kKept]);
       }
       tc_fence_before();
       mbar_arrive(&p_full[slot * 2 + (k & 1)]);
@@ -534,8 +563,8 @@ static cudaError_t launch_tc_typed(const CUtensorMap& map, const Attn8Params& p,
   const cudaError_t e = allow_smem(attn8_tc_kernel<T, kSplitKeys>, kSmem, done);
   if (e != cudaSuccess) return e;
   const int rows = p.M * (p.Hq / p.Hkv), tile = kSplitKeys ? 128 : 256;
-  return launch_k(attn8_tc_kernel<T, kSplitKeys>, dim3(p.Hkv, p.tc_splits, (rows + tile - 1) / tile), dim3(kThreads),
-                  kSmem, st, map, p);
+  return launch_k(attn8_tc_kernel<T, kSplitKeys>, dim3(p.Hkv, p.tc_splits, (rows + tile - 1) / tile), 
+                  dim3(Roles<kSplitKeys>::kThreads), kSmem, st, map, p);
 }
 
 cudaError_t launch_attention8_tc(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
