@@ -191,6 +191,26 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
   pdl_wait();
   pdl_trigger();  // after this CTA's TMEM allocation
 
+  // Q: an equal share of the rows per warp, a row per load of the whole warp (a thread per row would touch
+  // 32 lines with every load), eight rows at a time; the first eight are on their way before anything
+  // waits for memory.
+  constexpr int kQRows = ksplit ? 8 : 24;  // rows past the tile are not kept
+  int row = warp * kQRows, qm = (row0 + row) / G, qg = (row0 + row) - qm * G;
+  uint2 qraw[8];
+  auto load_q8 = [&]() {
+    const uint2* src = reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + h * G * kHd + lane * 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      qraw[i] = make_uint2(0, 0);
+      if (row + i < rows_cta) qraw[i] = src[(static_cast<int64_t>(qm) * p.Hq + qg) * (kHd / 4)];
+      if (++qg == G) {
+        qg = 0;
+        ++qm;
+      }
+    }
+  };
+  if (warp < R::kProducer) load_q8();
+
   // This split's chunks: up to the last key that any row of the CTA may see.
   const Attn8Shape sh = attn8_shape(p);
   int len_max = 0;
@@ -208,29 +228,13 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
   const int ps = 1 << p.page_shift;
 
   if (warp < R::kProducer) {
-    // Q: an equal share of the rows per warp, a row per load of the whole warp (a thread per row would touch
-    // 32 lines with every load), each row scaled by a power of two so that its largest element is in
-    // [1, 2), as fp16, swizzled.  Four rows at a time: code that runs once costs more to fetch than to
-    // run, and all sixteen rows unrolled took longer.
-    constexpr int kQRows = ksplit ? 8 : 24;  // rows past the tile are not kept
-    int row = warp * kQRows;
-    int qm = (row0 + row) / G, qg = (row0 + row) - qm * G;
-    const uint2* src = reinterpret_cast<const uint2*>(static_cast<const T*>(p.q) + h * G * kHd + lane * 4);
+    // Each row of Q scaled by a power of two so that its largest element is in [1, 2), as fp16, swizzled.
 #pragma unroll 1
-    for (int i0 = 0; i0 < kQRows; i0 += 4) {
-      uint2 w[4];
+    for (int i0 = 0; i0 < kQRows; i0 += 8) {
+      if (i0 > 0) load_q8();
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = make_uint2(0, 0);
-        if (row + i < rows_cta) w[i] = src[(static_cast<int64_t>(qm) * p.Hq + qg) * (kHd / 4)];
-        if (++qg == G) {
-          qg = 0;
-          ++qm;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i, ++row) {
-        const T* e = reinterpret_cast<const T*>(&w[i]);
+      for (int i = 0; i < 8; ++i, ++row) {
+        const T* e = reinterpret_cast<const T*>(&qraw[i]);
         const float q[4] = {to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
         const float am = fmaxf(max3(fabsf(q[0]), fabsf(q[1]), fabsf(q[2])), fabsf(q[3]));
         const int e2 = row_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(am)));
