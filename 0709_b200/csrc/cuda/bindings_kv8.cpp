@@ -17,6 +17,7 @@
 namespace {
 
 constexpr double kLog2e = 1.4426950408889634;
+constexpr int64_t kPositions = int64_t{1} << 30;  // positions and their differences fit 32 bits
 
 // Numbers in messages: streaming one into TORCH_CHECK from this extension ends the process (its copy of
 // the number formatting and torch's do not share their locale).
@@ -58,8 +59,7 @@ Cache8 check_cache(const torch::Tensor& data, const torch::Tensor& scale, int64_
 void check_int(const torch::Tensor& t, const torch::Tensor& like, const char* name, int64_t n = -1) {
   TORCH_CHECK(t.device() == like.device() && t.scalar_type() == torch::kInt32 && t.is_contiguous(), name,
               " must be a contiguous int32 tensor on the cache's device");
-  TORCH_CHECK(n < 0 || t.numel() == n, name, " must hold ", str(n), " values, not ",
-              str(t.numel()));
+  TORCH_CHECK(n < 0 || t.numel() == n, name, " must hold ", str(n), " values, not ", str(t.numel()));
 }
 
 void check_err(const torch::Tensor& err, const torch::Tensor& like) {
@@ -174,15 +174,23 @@ torch::Tensor kv8_read_pages(torch::Tensor data, torch::Tensor scale, int64_t la
   return out;
 }
 
-// The split pass's launch shape for `rows` query rows of a kv head (query rows times group).  Up to 32
-// rows go through the register tensor-core pass in tiles of 16 or 32 rows; more through the tcgen05
-// pass, whose CTA holds 128 rows over alternate chunks of keys or, above 128, 256 rows (8 kv heads, us:
-// 32 rows on 16K keys 24.8 against 28.5, 48 rows 34.6 against 29.9).  The splits fill the CTA slots
-// (two per SM for the small tile) with at least 128 keys each up to eight splits and 256 beyond (36
-// rows on 2051 keys: 17 splits 16.8 us, 9 splits 15.1 us; 48 rows on 1000 keys: 8 splits 10.9 us, 4
-// splits 12.4 us).
+// The split pass's launch shape for `rows` query rows of a kv head (query rows times group).
+//
+// The register tensor-core pass takes tiles of 16 rows (two CTAs per SM) or 32; its work is a term per tile
+// and key.  The tcgen05 pass holds 128 rows over alternate chunks of keys, or 256 rows, in a CTA: it starts
+// about 5 us later and then spends on all of its rows what the other spends on 2.5 tiles of 16.  Hence the
+// border: Hkv * keys * (tiles - 2.5) = 120 K (us, tiles of 16 against tcgen05; 8 kv heads: 48 rows on 4096
+// keys 13.9 / 17.4, on 16K 26.4 / 29.8, on 64K 75.9 / 66.6; 96 rows on 4096 18.0 / 18.0, on 8192 25.9 / 23.6;
+// 160 rows on 1024 13.6 / 15.9, on 4096 25.8 / 19.8; 16 kv heads, 320 rows on 300: 23.2 / 18.9, more CTAs
+// than fit at once).  Up to 32 rows it never pays, and one tile of 32 beats two of 16 from Hkv * keys = 128 K
+// on (8 kv heads, 20 rows: 4096 keys 12.8 / 11.9, 64K 50.1 / 54.9).
+//
+// The splits fill the CTA slots with at least 128 keys each up to eight splits and 256 beyond (36 rows on
+// 2051 keys: 17 splits 16.8 us, 9 splits 15.1 us; 48 rows on 1000 keys: 8 splits 10.9 us, 4 splits 12.4 us).
 void pick_shape8(atlas::Attn8Params& p, int64_t rows, int64_t keys, int sms) {
-  p.row_tile = p.causal_start >= 0 ? 0 : rows <= 16 ? 16 : rows <= 32 ? 32 : 0;
+  const int64_t tiles = (rows + 15) / 16, work = p.Hkv * keys;
+  const bool registers = tiles <= 2 || (work * (2 * tiles - 5) < 240 * 1024 && tiles * p.Hkv <= 2 * sms);
+  p.row_tile = p.causal_start >= 0 || !registers ? 0 : tiles == 2 && work >= 128 * 1024 ? 32 : 16;
   p.tc_ksplit = rows <= 128 ? 1 : 0;
   const int64_t tile = p.row_tile ? p.row_tile : p.tc_ksplit ? 128 : 256;
   const int64_t slots = static_cast<int64_t>(sms) * (p.row_tile == 16 ? 2 : 1);
@@ -226,7 +234,7 @@ void check_q8(torch::Tensor& q, const torch::Tensor& data, const Cache8& c, doub
 }
 
 atlas::Attn8Params params8(const torch::Tensor& q, const Cache8& c, const torch::Tensor& out,
-const torch::Tensor& prefix_pages, double softmax_scale, const torch::Tensor& err) {
+                            const torch::Tensor& prefix_pages, double softmax_scale, const torch::Tensor& err) {
   atlas::Attn8Params p{};
   p.q = q.data_ptr();
   p.data = c.data;
@@ -246,11 +254,13 @@ const torch::Tensor& prefix_pages, double softmax_scale, const torch::Tensor& er
   return p;
 }
 
-std::pair<torch::Tensor, int64_t> attention8(
-                         torch::Tensor q, torch::Tensor data, torch::Tensor scale, int64_t layer,
-                         c10::optional<torch::Tensor> dparams, int64_t shared_len, int64_t n_shared_pages, int64_t mask_base, torch::Tensor prefix_pages,
-                         torch::Tensor row_full, torch::Tensor row_len, torch::Tensor row_mask, torch::Tensor tail_pages,
-                         double softmax_scale, int64_t max_keys, torch::Tensor err) {
+// Returns the output and the number of kernels launched.
+std::pair<torch::Tensor, int64_t> attention8(torch::Tensor q, torch::Tensor data, torch::Tensor scale, int64_t layer,
+                                             c10::optional<torch::Tensor> dparams, int64_t shared_len,
+                                             int64_t n_shared_pages, int64_t mask_base, torch::Tensor prefix_pages,
+                                             torch::Tensor row_full, torch::Tensor row_len, torch::Tensor row_mask,
+                                             torch::Tensor tail_pages, double softmax_scale, int64_t max_keys,
+                                             torch::Tensor err) {
   TORCH_CHECK(layer >= 0, "layer ", str(layer));
   const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
@@ -264,11 +274,13 @@ std::pair<torch::Tensor, int64_t> attention8(
               "row_mask must be contiguous int64 [M, words] on the cache's device");
   check_int(tail_pages, data, "tail_pages");
   TORCH_CHECK(tail_pages.dim() == 2 && tail_pages.size(0) == M, "tail_pages must be [M, T]");
-  TORCH_CHECK((prefix_pages.numel() << c.shift) < (1 << 30) &&
-                  ((n_shared_pages + tail_pages.size(1)) << c.shift) < (1 << 30),
-              "the descriptor's page lists must end below position 2^30");
-  TORCH_CHECK(shared_len >= 0 && n_shared_pages >= 0 && std::max(shared_len, n_shared_pages << c.shift) < (1 << 30),
+  TORCH_CHECK(shared_len >= 0 && shared_len < kPositions && n_shared_pages >= 0 &&
+                  n_shared_pages < (kPositions >> c.shift),
               "shared_len and n_shared_pages must be positions below 2^30");
+  TORCH_CHECK((prefix_pages.numel() << c.shift) < kPositions &&
+                  ((n_shared_pages + tail_pages.size(1)) << c.shift) < kPositions,
+              "the descriptor's page lists must end below position 2^30");
+  TORCH_CHECK(mask_base > -kPositions && mask_base < kPositions, "mask_base must be a position below 2^30");
   if (dparams.has_value()) {
     check_int(*dparams, data, "the descriptor's device scalars");
     TORCH_CHECK(dparams->numel() >= 3, "the descriptor's device scalars are shared_len, n_shared_pages, mask_base");
@@ -300,15 +312,16 @@ std::pair<torch::Tensor, int64_t> attention8(
 }
 
 // Row m is at position start + m and sees the keys up to itself, all in prefix_pages.
-std::pair<torch::Tensor, int64_t> attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tensor scale, int64_t layer,
-                                torch::Tensor prefix_pages, int64_t start, double softmax_scale, torch::Tensor err) {
+std::pair<torch::Tensor, int64_t> attention8_causal(torch::Tensor q, torch::Tensor data, torch::Tensor scale,
+                                                    int64_t layer, torch::Tensor prefix_pages, int64_t start,
+                                                    double softmax_scale, torch::Tensor err) {
   TORCH_CHECK(layer >= 0, "layer ", str(layer));
   const Cache8 c = check_cache(data, scale, layer);
   check_err(err, data);
   check_q8(q, data, c, softmax_scale);
   check_int(prefix_pages, data, "prefix_pages");
   const int64_t M = q.size(0), ps = c.ps;
-  TORCH_CHECK(start >= 0 && start + M < (1 << 30), "positions must be in [0, 2^30)");
+  TORCH_CHECK(start >= 0 && start < kPositions && start + M < kPositions, "positions must be in [0, 2^30)");
   const int64_t n = (start + M + ps - 1) / ps;
   TORCH_CHECK(n <= prefix_pages.numel(), str(start + M), " positions need ", str(n), " pages of ", str(ps),
               " slots; the descriptor lists ", str(prefix_pages.numel()));

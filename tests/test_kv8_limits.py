@@ -2,13 +2,14 @@
 
 from __future__ import annotations
 
+import dataclasses
 import math
 
 import pytest
 import torch
 
 from conftest import mod
-from test_kv8 import Oracle, assert_pages, check_attention, impl, make_cache, make_desc, rope, settle
+from test_kv8 import ATTENTIONS, Oracle, assert_pages, check_attention, impl, make_cache, make_desc, rope, settle
 
 IMPLS = [pytest.param("cpu", id="cpu"), pytest.param("cuda", id="cuda", marks=pytest.mark.gpu)]
 
@@ -165,6 +166,12 @@ def test_calls_that_are_refused():
         lambda: ops.attention8(q, make_cache("cuda", 1, 6, 2, 4, 128, seed=0).layer(0), desc),
         lambda: ops.attention8_causal(q, layer, desc, -1),
         lambda: ops.attention8_causal(q, layer, desc, 31),
+        lambda: ops.attention8_causal(q, layer, desc, 2 ** 63 - 1),
+        lambda: ops.attention8_causal(q, layer, desc, 2 ** 32),
+        lambda: ops.attention8(q, layer, dataclasses.replace(desc, n_shared_pages=2 ** 62)),
+        lambda: ops.attention8(q, layer, dataclasses.replace(desc, n_shared_pages=-1)),
+        lambda: ops.attention8(q, layer, dataclasses.replace(desc, shared_len=2 ** 32 + 5)),
+        lambda: ops.attention8(q, layer, dataclasses.replace(desc, mask_base=2 ** 32)),
         lambda: ops.rope_qkv_append8(qkv, table, one, one, layer, 2, 1),
         lambda: ops.rope_qkv_append8(qkv, table, one, one, layer, 3, 2),
         lambda: ops.rope_qkv_append8(qkv, table, one, one, layer, 2, 2, out_dtype=torch.bfloat16),
@@ -207,6 +214,43 @@ def test_empty_calls():
 
 
 # ------------------------------------------------------------ long and wide
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind,ps,hq,hkv,length,rows", ATTENTIONS)
+def test_attention_sized_for_a_longer_context(dtype, kind, ps, hq, hkv, length, rows):
+    """Short contexts in the launch shape of a captured graph that may see 2^20 keys: the pass for long sequences, and
+    splits that have no key."""
+    ops = impl("cuda")
+    pages = 4 + -(-(length + rows + 1) // ps) + (rows * 2 if kind == "routes" else 0)
+    desc = make_desc("cuda", kind, ps, length, rows, seed=length + rows, pages=pages)
+    desc._max_keys = 1 << 20
+    cache = make_cache("cuda", 2, pages, hkv, ps, 128, seed=length)
+    q = torch.randn(rows, hq, 128, generator=torch.Generator().manual_seed(rows)).to(dtype)
+    out = ops.attention8(q.cuda(), cache.layer(1), desc)
+    settle(ops)
+    check_attention(out, q, Oracle(cache).val[1], desc, 1 / math.sqrt(128))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,hq,hkv,length,rows", [
+    ("tree", 4, 1, 700, 9), ("tree", 8, 1, 1500, 33), ("ragged", 32, 2, 900, 12), ("routes", 8, 2, 1031, 30),
+    ("tree", 128, 1, 333, 5), ("ragged", 12, 3, 20000, 5)])
+def test_attention_at_more_row_tiles(kind, hq, hkv, length, rows):
+    """Several tiles of 16 rows over the same keys, and the other side of the border between the passes."""
+    ops = impl("cuda")
+    pages = 4 + -(-(length + rows + 1) // 16) + (rows * 2 if kind == "routes" else 0)
+    desc = make_desc("cuda", kind, 16, length, rows, seed=length, pages=pages)
+    cache = make_cache("cuda", 1, pages, hkv, 16, 128, seed=length)
+    q = torch.randn(rows, hq, 128, generator=torch.Generator().manual_seed(rows)).half()
+    outs = []
+    for keys in (0, 1 << 20):
+        desc._max_keys = keys
+        outs.append(ops.attention8(q.cuda(), cache.layer(0), desc))
+    settle(ops)
+    for out in outs:
+        check_attention(out, q, Oracle(cache).val[0], desc, 1 / math.sqrt(128))
+
+
 def torch_attention(q, values, pages, lens, scale):
     """float64 on the GPU, rows that see a prefix of one page list."""
     m, hq, hd = q.shape
@@ -227,7 +271,7 @@ def torch_attention(q, values, pages, lens, scale):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("hq,hkv,rows,length", [(32, 32, 1, 80003), (64, 32, 16, 40001), (32, 2, 3, 60000),
-                                                (16, 2, 33, 50001)])
+                                                (16, 2, 33, 50001), (32, 2, 6, 60000)])
 def test_attention_over_long_sequences(hq, hkv, rows, length):
     """Many pages per warp and CTA (rings and page windows wrap), for each of the three passes."""
     ops, kv8, attn_desc = impl("cuda"), mod("ops.kv8"), mod("ops.attn_desc")
