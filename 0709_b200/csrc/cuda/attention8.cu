@@ -42,7 +42,7 @@ __device__ __forceinline__ void fold_tail8(const Attn8Params& p, const Attn8Shap
         set_error(p.err, kErrBadIndex);
       } else {
         ph = static_cast<int64_t>(page) * 2 * p.Hkv + h;
-        sc = attn8_scales(p, ph);
+        sc = attn8_scales(p.scale[ph], p.scale[ph + p.Hkv]);
       }
     }
     const int cnt = min(32, x1 - t0);

@@ -32,10 +32,9 @@ __device__ __forceinline__ int attn8_end(const Attn8Params& p, const Attn8Shape&
   return min(end, listed);
 }
 
-// Scales of a page and head as the kernels use them: k scale, log2(v scale), 1 / v scale.  An empty
+// Scales of a page and head (k and v) as the kernels use them: k scale, log2(v scale), 1 / v scale.  An empty
 // page (scale 0) holds zero codes: any positive scale reads it right.
-__device__ __forceinline__ float4 attn8_scales(const Attn8Params& p, int64_t page_head) {
-  const float k = p.scale[page_head], v = p.scale[page_head + p.Hkv];
+__device__ __forceinline__ float4 attn8_scales(float k, float v) {
   const int e = v > 0.f ? static_cast<int>(__float_as_uint(v) >> 23) - 127 : 0;
   return make_float4(k > 0.f ? k : 1.f, static_cast<float>(e), __int_as_float((127 - e) << 23), 0.f);
 }

@@ -11,10 +11,16 @@
 //         P V tiles whose products take 1280).
 // S is double-buffered in TMEM, so that a slot's next scores are ready when its softmax is; P (fp16)
 // replaces its S in place and is the A operand of O += P V.  Q is read from shared memory (TMEM has no
-// room left).  Per 64-key chunk the shared memory carries the codes (16 KB written, 16 KB read), the
-// fp16 tiles (32 KB written) and per slot 16 KB of K, 32 KB of Q and 16 KB of V.
+// room left; a form with Q and P in TMEM and a single S took 362 us where this one took 306).
 //
 // TMEM columns: S/P of slot s, buffer b at 128 s + 64 b; O of slot s at 256 + 128 s.
+//
+// Measured: 2048 rows x 32 heads behind 6001 keys (8 kv heads) 259 us, 0.57 of the measured bf16 matrix rate;
+// 192 rows a head on 16384 keys 34.8 us and 104 rows on 33001 keys 41.8 us with the merge.  What bounds it,
+// from cycle stamps of the first: a chunk takes 2120 cycles; the tensor pipe works for 1580 of them (an S
+// product of 64 keys reads 6 KB of shared memory and runs at half rate: 65 cycles for 32), a softmax warp for
+// 1750 (two share a scheduler), the converters for 880.  The short calls are bound by their start: a CTA's
+// first scores come about 6000 cycles after its launch, O leaves 2000 after its last chunk.
 
 #include "attention8.cuh"
 
@@ -22,23 +28,27 @@ namespace atlas {
 
 namespace {
 constexpr int kChunk = 64;
-constexpr int kStages8 = 4;                    // chunks of codes in flight
 constexpr int kBytes8 = kChunk * kHd * 2;      // K | V codes
 constexpr int kHalf16 = kChunk * 128;          // 64 keys x 64 dimensions of fp16
 constexpr int kBytes16 = 4 * kHalf16;          // K halves | V halves
 constexpr int kBytesQ = 128 * kHd * 2;         // two halves of 128 rows x 128 B
-static_assert(256 * (kHd * 4 + 16) <= kStages8 * kBytes8 + 4 * kBytes16, "the output rows reuse the chunks' space");
-static_assert(kBytesQ == kBytes16, "slot 1's own Q takes the place of the fourth converted chunk");
-// Converter groups of four warps: with split keys a chunk feeds one slot only and two groups keep up.
+constexpr int kStages16 = 4;  // converted chunks
+static_assert(256 * (kHd * 4 + 16) <= 2 * kBytes8 + kStages16 * kBytes16, "the output rows reuse the chunks' space");
+static_assert(kBytesQ == 2 * kBytes8, "slot 1's own Q takes the place of two chunks of codes");
+// Converter groups of four warps: with split keys a chunk feeds one slot only and two groups keep up.  Where
+// both slots share the chunks, a fourth converted one is worth more than two more chunks of codes (the slots
+// need not keep step: 265 -> 259 us); with split keys six chunks of codes and three converted took 45.7 us
+// for 42.3.
 template <bool kSplitKeys>
 struct Roles {
+  static constexpr int kStages8 = kSplitKeys ? 4 : 2;  // chunks of codes in flight
   static constexpr int kConvGroups = kSplitKeys ? 2 : 1;
   static constexpr int kProducer = 8 + 4 * kConvGroups;
   static constexpr int kThreads = (kProducer + 3) * 32;
 };
-constexpr int kSmem = 1024 + kStages8 * kBytes8 + 4 * kBytes16 + kBytesQ + (kStages8 + 4) * 128 + 256 + 256;
+constexpr int kSmem = 1024 + 4 * kBytes8 + kStages16 * kBytes16 + kBytesQ + (4 + kStages16) * 128 + 256 + 256;
 constexpr uint32_t kColO = 256;
-constexpr float kGrow = 8.f;  // log2: P stays <= 256 between rescales
+constexpr float kGrow = 14.f;  // log2: P stays <= 2^14 between rescales (fp16 ends at 2^16)
 }  // namespace
 
 // D (+)= A(tmem) * B(smem); B's descriptor as two words, so that the tiles of one operand differ by
@@ -127,20 +137,22 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
-template <typename T, bool kSplitKeys>
+// kGroup: keys that share their scales, 8 or 16 (pages of 8 slots, or more).  Groups of 16 halve the scale
+// reads and their arithmetic: 279 -> 265 us.
+template <typename T, bool kSplitKeys, int kGroup>
 __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
     attn8_tc_kernel(const __grid_constant__ CUtensorMap map, Attn8Params p) {
   constexpr bool ksplit = kSplitKeys;
   using R = Roles<kSplitKeys>;
-  constexpr int kStages16 = kSplitKeys ? 4 : 3;  // converted chunks
+  constexpr int kStages8 = R::kStages8;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* ring8 = smem;
   uint8_t* ring16 = ring8 + kStages8 * kBytes8;
-  uint8_t* q_s = ring16 + 4 * kBytes16;  // slot 0 (and both slots with split keys)
-  uint8_t* q1_s = ring16 + 3 * kBytes16;
+  uint8_t* q_s = ring16 + kStages16 * kBytes16;  // slot 0 (and both slots with split keys)
+  uint8_t* q1_s = q_s + kBytesQ;
   // Per 8 keys of a chunk: k scale, log2(v scale), 1 / v scale.
-  float4* sc8 = reinterpret_cast<float4*>(q_s + kBytesQ);  // [kStages8][8]
+  float4* sc8 = reinterpret_cast<float4*>(q_s + (ksplit ? 1 : 2) * kBytesQ);  // [kStages8][8]
   float4* sc16 = sc8 + kStages8 * 8;                                       // [kStages16][8]
   uint64_t* full8 = reinterpret_cast<uint64_t*>(sc16 + 4 * 8);
   uint64_t* empty8 = full8 + kStages8;
@@ -253,54 +265,68 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
   }
 
   if (warp == R::kProducer) {
-    // ---- producer.  Lane l holds page and scales of 8 keys, l & 7, of chunk l >> 3 of a window of
-    // four; the next window is loaded while this one is issued (page and scale are two dependent
-    // trips to memory: taken chunk by chunk they bound the pass at 2 TB/s).
+    // ---- producer.  Lane l holds page and scales of 8 keys, l & 7, of chunk l >> 3 of a window of four.
+    // A chunk's copies need its pages, which are read two windows ahead; the scales, another dependent trip to
+    // memory, are read one window ahead and handed over after the copies are issued.
     const int box = min(ps, 16);
-    struct Window {
-      int page;
-      float4 sc;
-    };
-    auto load_window = [&](int first) {
-      Window w{0, make_float4(1.f, 0.f, 1.f, 0.f)};
+    constexpr int kNone = -1;  // no key of this split
+    auto load_page = [&](int first) {
       const int c = first + (lane >> 3), x = (c0 + c) * kChunk + (lane & 7) * 8;
-      if (c < chunks && x < end) {
-        const int page = p.prefix_pages[x >> p.page_shift];
-        if (page < 0 || page >= p.num_pages) {
-          set_error(p.err, kErrBadIndex);
-        } else {
-          w.page = page;
-          w.sc = attn8_scales(p, static_cast<int64_t>(page) * 2 * p.Hkv + h);
-        }
-      }
-      return w;
+      return c < chunks && x < end ? p.prefix_pages[x >> p.page_shift] : kNone;
     };
-    Window cur = load_window(0), nxt = load_window(4);
-    for (int c = 0; c < chunks; ++c) {
-      if (c > 0 && (c & 3) == 0) {
-        cur = nxt;
-        nxt = load_window(c + 4);
+    struct Scales {
+      float k, v;
+    };
+    // Sets a page that is not of the cache to kNone after reporting it; its keys read as page 0 does.
+    auto load_scales = [&](int& page, int first) {
+      if (page < 0 || page >= p.num_pages) {
+        const int c = first + (lane >> 3), x = (c0 + c) * kChunk + (lane & 7) * 8;
+        if (c < chunks && x < end) set_error(p.err, kErrBadIndex);
+        page = kNone;
       }
-      const int s = c % kStages8, from = (c & 3) * 8 + (lane & 7);
-      const int page = __shfl_sync(0xffffffffu, cur.page, from);
-      float4 sc;
-      sc.x = __shfl_sync(0xffffffffu, cur.sc.x, from);
-      sc.y = __shfl_sync(0xffffffffu, cur.sc.y, from);
-      sc.z = __shfl_sync(0xffffffffu, cur.sc.z, from);
-      sc.w = 0.f;
-      bool ok = c < kStages8 || wait8(&empty8[s], ((c / kStages8) - 1) & 1, p.err);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane < 8) sc8[s * 8 + lane] = sc;
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(&full8[s], kBytes8);
-      __syncwarp();
-      // Lane g < 8 issues the box that starts at its 8 keys (every other lane when a box holds 16).
+      Scales r{0.f, 0.f};
+      if (page != kNone) {
+        const float* f = p.scale + static_cast<int64_t>(page) * 2 * p.Hkv + h;
+        r.k = f[0];
+        r.v = f[p.Hkv];
+      }
+      return r;
+    };
+    // Lane g < 8 issues the box that starts at its 8 keys (every other lane when a box holds 16).
+    auto issue = [&](int c, int window_page) {
+      const int page = max(0, __shfl_sync(0xffffffffu, window_page, (c & 3) * 8 + (lane & 7)));
+      const int s = c % kStages8;
       if (lane < 8 && (box == 8 || (lane & 1) == 0)) {
         const int y = (page * 2 * p.Hkv + h) * ps + (((c0 + c) * kChunk + lane * 8) & (ps - 1));
         uint8_t* dst = ring8 + s * kBytes8 + lane * 8 * kHd;
         tma_load_2d(dst, &map, &full8[s], 0, y);
         tma_load_2d(dst + kBytes8 / 2, &map, &full8[s], 0, y + p.Hkv * ps);
       }
+    };
+    int page = load_page(0), next_page = load_page(4), far_page = load_page(8);
+    Scales cur = load_scales(page, 0);
+    for (int c = 0; c < min(chunks, kStages8); ++c) issue(c, page);
+    Scales next = load_scales(next_page, 4);
+    for (int c = 0; c < chunks; ++c) {
+      if (c > 0 && (c & 3) == 0) {
+        page = next_page;
+        cur = next;
+        next_page = far_page;
+        next = load_scales(next_page, c + 4);
+        far_page = load_page(c + 8);
+      }
+      const int s = c % kStages8;
+      if (c >= kStages8) {
+        const bool ok = wait8(&empty8[s], ((c / kStages8) - 1) & 1, p.err);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        issue(c, page);
+      }
+      const float k = __shfl_sync(0xffffffffu, cur.k, (c & 3) * 8 + (lane & 7));
+      const float v = __shfl_sync(0xffffffffu, cur.v, (c & 3) * 8 + (lane & 7));
+      if (lane < 8) sc8[s * 8 + lane] = attn8_scales(k, v);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(&full8[s], kBytes8);
+      __syncwarp();
     }
   } else if (warp >= 8 && warp < R::kProducer) {
     // ---- converters: one 16-byte piece of codes (16 dimensions of a key) per thread and step
@@ -438,9 +464,11 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
       };
       auto half_top = [&](int half, const float* v) {
 #pragma unroll
-        for (int gk = 0; gk < 4; ++gk, v += 8) {
+        for (int gk = 0; gk < 4; gk += kGroup / 8, v += kGroup) {
           const float4 w = sc[half * 4 + gk];
-          const float mx = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
+          float mx = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
+          if constexpr (kGroup == 16)
+            mx = max3(mx, max3(max3(v[8], v[9], v[10]), v[11], v[12]), max3(v[13], v[14], v[15]));
           top = fmaxf(top, fmaf(mx, fac * w.x, w.y));
         }
       };
@@ -483,12 +511,12 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
       auto weigh_half = [&](int half, const float* v) {
         float pk[16];
 #pragma unroll
-        for (int gk = 0; gk < 4; ++gk) {
+        for (int gk = 0; gk < 4; gk += kGroup / 8) {
           const float4 w = sc[half * 4 + gk];
           const uint64_t f = pair2(fac * w.x, fac * w.x), b = pair2(w.y + neg, w.y + neg);
           uint64_t acc = 0;
 #pragma unroll
-          for (int j = 0; j < 8; j += 2) {
+          for (int j = 0; j < kGroup; j += 2) {
             float p0, p1;
             unpair2(fma2(pair2(v[gk * 8 + j], v[gk * 8 + j + 1]), f, b), p0, p1);
             p0 = ex2(p0);
@@ -561,14 +589,20 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 
-template <typename T, bool kSplitKeys>
-static cudaError_t launch_tc_typed(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
+template <typename T, bool kSplitKeys, int kGroup>
+static cudaError_t launch_tc_grouped(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_smem(attn8_tc_kernel<T, kSplitKeys>, kSmem, done);
+  const cudaError_t e = allow_smem(attn8_tc_kernel<T, kSplitKeys, kGroup>, kSmem, done);
   if (e != cudaSuccess) return e;
   const int rows = p.M * (p.Hq / p.Hkv), tile = kSplitKeys ? 128 : 256;
-  return launch_k(attn8_tc_kernel<T, kSplitKeys>, dim3(p.Hkv, p.tc_splits, (rows + tile - 1) / tile), 
+  return launch_k(attn8_tc_kernel<T, kSplitKeys, kGroup>, dim3(p.Hkv, p.tc_splits, (rows + tile - 1) / tile),
                   dim3(Roles<kSplitKeys>::kThreads), kSmem, st, map, p);
+}
+
+template <typename T, bool kSplitKeys>
+static cudaError_t launch_tc_typed(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
+  return p.page_shift == 3 ? launch_tc_grouped<T, kSplitKeys, 8>(map, p, st)
+                           : launch_tc_grouped<T, kSplitKeys, 16>(map, p, st);
 }
 
 cudaError_t launch_attention8_tc(const CUtensorMap& map, const Attn8Params& p, cudaStream_t st) {
