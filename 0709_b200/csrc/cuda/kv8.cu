@@ -123,7 +123,7 @@ __device__ __forceinline__ void load_kv8(const Kv8AppendParams& p, int r, int po
 
 // One kv head of `page`, which row m writes, if m is the first row of the batch to write it: all of the
 // page's rows.  So each page and head has one writer and no order of blocks matters.
-template <typename T>
+template <typename T, bool kDense>
 __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int page, int h) {
   __shared__ int owner[kMaxPage];  // row that writes slot o, -1: none
   __shared__ uint32_t amax_s[2];
@@ -159,7 +159,7 @@ __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int
   // left out.
   const int i = (lane & 15) * 4, sub = lane >> 4;
   uint32_t ak = 0, av = 0;
-#pragma unroll 2
+#pragma unroll (kDense ? 1 : 2)
   for (int o2 = warp * 2; o2 < ps; o2 += 8) {
     const int o = o2 + sub, r = owner[o];
     const int pos = r >= 0 ? p.pos[r] : -1;
@@ -198,7 +198,7 @@ __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int
   const float inv_k = 1.f / new_k, inv_v = 1.f / new_v;
   uint32_t* kd = reinterpret_cast<uint32_t*>(p.data) + ((static_cast<int64_t>(page) * 2) * p.Hkv + h) * ps * (kHd / 4);
   uint32_t* vd = kd + static_cast<int64_t>(p.Hkv) * ps * (kHd / 4);
-#pragma unroll 2
+#pragma unroll (kDense ? 1 : 2)
   for (int o2 = warp * 2; o2 < ps; o2 += 8) {
     const int o = o2 + sub, r = owner[o];
     uint32_t* ko = kd + o * (kHd / 4) + i / 4;  // words of dimensions i and 64 + i: 16 apart
@@ -230,8 +230,11 @@ __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int
 
 // 128 threads.  The first q_blocks blocks rotate Q, q_per_warp (row, head) pairs per warp; the others
 // take kv_rows consecutive rows of one kv head each and write the pages that these rows start.
-template <typename T, typename O>
-__global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
+// Few rows are bound by latency: launch, slots, then the rows and the page they meet (one row 4.4 us, 13
+// rows 4.9 us, 32 / 8 heads).  A prompt is bound by bytes and by the two reads of each row, for the maximum
+// and for the codes (the second one hits the L1 or L2): 5001 rows of bf16 30 us for 113 MB.
+template <typename T, typename O, bool kDense>
+__device__ __forceinline__ void append_body(const Kv8AppendParams& p) {
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -240,7 +243,7 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
     uint32_t pair = (blockIdx.x * 4 + warp) * p.q_per_warp + (lane >> 4);  // 16 lanes each
     const uint32_t stop = min(pairs, (blockIdx.x * 4 + warp + 1) * p.q_per_warp);
     const int i = (lane & 15) * 4;
-#pragma unroll 4
+#pragma unroll (kDense ? 2 : 4)
     for (; pair < stop; pair += 2) {
       const int m = pair / static_cast<uint32_t>(p.Hq), head = pair - m * p.Hq;
       const int pos = p.pos[m];
@@ -270,11 +273,22 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
   while (todo) {
     const int i = __ffs(todo) - 1;
     todo &= todo - 1;
-    append_page<T>(p, m0 + i, __shfl_sync(0xffffffffu, page, i), h);
+    append_page<T, kDense>(p, m0 + i, __shfl_sync(0xffffffffu, page, i), h);
   }
 }
 
-// grid (min(n, 64), layers, 2 * Hkv).  Copies of one call are independent: a destination that is
+template <typename T, typename O>
+__global__ void __launch_bounds__(128) kv8_append_kernel(Kv8AppendParams p) {
+  append_body<T, O, false>(p);
+}
+template <typename T, typename O>
+__global__ void __launch_bounds__(128, 12) kv8_append_dense_kernel(Kv8AppendParams p) {
+  append_body<T, O, true>(p);
+}
+
+// grid (min(n, 64), layers, 2 * Hkv): one page and head per block and step, 2 KB for 16 slots, so that a
+// fork of a few pages spreads over the device (9 pages in 16 layers, 8 kv heads: 6.5 us for 9.4 MB read and
+// written, launch included).  Copies of one call are independent: a destination that is
 // also a source, or twice a destination, is reported and skipped.  The slots behind the copied ones
 // are zeroed; a copy of no token leaves an empty page (scale 0), which is how a page is freed.
 __global__ void __launch_bounds__(128)
@@ -305,7 +319,8 @@ __global__ void __launch_bounds__(128)
 }
 
 // grid (layers, 2 * Hkv), 256 threads; shared memory: n codes rows, scales, slots, page tables.
-// Every source is read before any slot is written; then one warp per destination page.
+// Every source is read before any slot is written; then one warp per destination page, which may have to
+// round its other slots again.  Bound by latency, three dependent trips to memory (4 moves in 32 layers 7.3 us).
 __global__ void __launch_bounds__(256)
     kv8_move_slots_kernel(uint8_t* __restrict__ data, float* __restrict__ scale, const int* __restrict__ src,
                           const int* __restrict__ dst, int n, int num_pages, int Hkv, int page_shift, int* err) {
@@ -382,7 +397,8 @@ __device__ __forceinline__ __nv_bfloat16 kv8_value<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// grid (n, layers, 2 * Hkv): one page and head, 16 codes per thread and step.  fp16 values are held
+// grid (n, layers, 2 * Hkv): one page and head, 16 codes per thread and step; bound by the bytes written (313
+// pages of 16 x 8 heads: 9.1 us for 31 MB, L2 cold).  fp16 values are held
 // to its largest finite number (rounding up to e4m3 can pass it).
 template <typename O>
 __global__ void __launch_bounds__(128)
@@ -419,21 +435,29 @@ __global__ void __launch_bounds__(128)
   }
 }
 
+template <typename T, typename O>
+static cudaError_t launch_append(const Kv8AppendParams& p, bool dense, dim3 grid, cudaStream_t st) {
+  return launch_k(dense ? kv8_append_dense_kernel<T, O> : kv8_append_kernel<T, O>, grid, dim3(128), 0, st, p);
+}
+
 cudaError_t launch_kv8_append(const Kv8AppendParams& params, cudaStream_t st) {
   if (params.M == 0) return cudaSuccess;
   // Few rows: every (row, head) on a warp of its own, for latency.  Many: blocks of one such piece each
-  // spend their time starting (98 us for 5001 rows); 8 pairs per warp and 16 rows per page block.
+  // spend their time starting (98 us for 5001 rows); 8 pairs per warp and 16 rows per page block.  From 64 K
+  // (row, head) pairs on, 32 pairs per warp and 40 registers for 12 blocks per SM (39 us where the form with
+  // 64 registers took 48; 1200 rows 16.3 us in both, 300 rows 7.5 in this one and 8.1 in that).
   Kv8AppendParams p = params;
-  p.q_per_warp = p.M > 64 ? 8 : 2;
+  const bool dense = static_cast<int64_t>(p.M) * p.Hq >= 65536;
+  p.q_per_warp = dense ? 32 : p.M > 64 ? 8 : 2;
   p.kv_rows = p.M > 64 ? 16 : 1;
   const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
   const int64_t per_block = 4 * p.q_per_warp;
   p.q_blocks = static_cast<int>((pairs + per_block - 1) / per_block);
   const dim3 grid(p.q_blocks + (p.M + p.kv_rows - 1) / p.kv_rows * p.Hkv);
-  if (p.in_type == kKv8Bf16) return launch_k(kv8_append_kernel<__nv_bfloat16, __nv_bfloat16>, grid, dim3(128), 0, st, p);
-  if (p.in_type == kKv8F16) return launch_k(kv8_append_kernel<__half, __half>, grid, dim3(128), 0, st, p);
-  if (p.out_bf16) return launch_k(kv8_append_kernel<float, __nv_bfloat16>, grid, dim3(128), 0, st, p);
-  return launch_k(kv8_append_kernel<float, __half>, grid, dim3(128), 0, st, p);
+  using B = __nv_bfloat16;
+  if (p.in_type == kKv8Bf16) return launch_append<B, B>(p, dense, grid, st);
+  if (p.in_type == kKv8F16) return launch_append<__half, __half>(p, dense, grid, st);
+  return p.out_bf16 ? launch_append<float, B>(p, dense, grid, st) : launch_append<float, __half>(p, dense, grid, st);
 }
 
 cudaError_t launch_kv8_copy_pages(uint8_t* data, float* scale, const int* plan, const int* count, int n, int layers,

@@ -329,8 +329,8 @@ class CudaOps:
         scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
         out, launches = self.ext.attention8(
             q, kv_layer.cache.data, kv_layer.cache.scale, kv_layer.index, getattr(desc, "_dparams", None),
-            desc.shared_len, desc.n_shared_pages, desc.mask_base, desc.prefix_pages, desc.row_full, desc.row_len, desc.row_mask, desc.tail_pages, scale,
-            getattr(desc, "_max_keys", 0), self.err,
+            desc.shared_len, desc.n_shared_pages, desc.mask_base, desc.prefix_pages, desc.row_full, desc.row_len,
+            desc.row_mask, desc.tail_pages, scale, getattr(desc, "_max_keys", 0), self.err,
         )
         counters.launches(launches)
         return out

@@ -314,20 +314,24 @@ def test_many_moves(moves):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [65, 700])
-def test_append_of_many_rows_in_any_order(rows):
-    """More rows than the latency form takes, shuffled over the pages, some slots named twice."""
+@pytest.mark.parametrize("rows,hq,dtype", [(65, 3, torch.bfloat16), (700, 3, torch.bfloat16), (2100, 32, torch.float16),
+                                           (2049, 32, torch.float32)])
+def test_append_of_many_rows_in_any_order(rows, hq, dtype):
+    """More rows than the latency form takes, shuffled over the pages, some slots named twice; from 64 K (row, head)
+    pairs on in the form for long prompts."""
     ops = impl("cuda")
-    cache = make_cache("cuda", 1, 60, 2, 16, 128, seed=rows)
+    pages = 60 if rows < 960 else 140
+    cache = make_cache("cuda", 1, pages, 2, 16, 128, seed=rows)
     other = mod("ops.kv8").Kv8Cache(cache.data.cpu(), cache.scale.cpu())
     g = torch.Generator().manual_seed(rows)
-    slots = torch.randperm(960, generator=g)[:rows].int()
+    slots = torch.randperm(pages * 16, generator=g)[:rows].int()
     slots[3] = slots[rows - 2]
-    qkv = torch.randn(rows, 7 * 128, generator=g).bfloat16()
+    qkv = torch.randn(rows, (hq + 4) * 128, generator=g).to(dtype)
     pos = torch.zeros(rows, dtype=torch.int32)  # the rotation is the identity: no value is next to a border by rounding
     table = rope(4, 128, "cpu")
-    q = ops.rope_qkv_append8(qkv.cuda(), table.cuda(), pos.cuda(), slots.cuda(), cache.layer(0), 3, 2)
-    want = mod("ops.torch_ops").rope_qkv_append8(qkv, table, pos, slots, other.layer(0), 3, 2)
+    out = torch.float16 if dtype == torch.float32 else dtype
+    q = ops.rope_qkv_append8(qkv.cuda(), table.cuda(), pos.cuda(), slots.cuda(), cache.layer(0), hq, 2, out_dtype=out)
+    want = mod("ops.torch_ops").rope_qkv_append8(qkv, table, pos, slots, other.layer(0), hq, 2, out_dtype=out)
     settle(ops)
     assert torch.equal(q.cpu(), want)
     assert torch.equal(cache.scale.cpu(), other.scale)
