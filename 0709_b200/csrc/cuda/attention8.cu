@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
       if (two) {
         const int zk = ((pb * 2) * p.Hkv + h) * ps;
         tma_load_2d(dst + 1024, &map, &bar[s], 0, zk);
-        tma_load_2d(dst + 3072, &map, &bar[s], 0, zk + p.Hkv * ps);
+        tma_load_2d(dst + 2048 + 1024, &map, &bar[s], 0, zk + p.Hkv * ps);
       }
     }
   };

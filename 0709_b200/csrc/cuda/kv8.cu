@@ -231,7 +231,7 @@ __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int
 // 128 threads.  The first q_blocks blocks rotate Q, q_per_warp (row, head) pairs per warp; the others
 // take kv_rows consecutive rows of one kv head each and write the pages that these rows start.
 // Few rows are bound by latency: launch, slots, then the rows and the page they meet (one row 4.4 us, 13
-// rows 4.9 us, 32 / 8 heads).  A prompt is bound by bytes and by the two reads of each row, for the maximum
+// rows 4.9 us with the pages read back, 32 / 8 heads).  A prompt is bound by bytes and by the two reads of each row, for the maximum
 // and for the codes (the second one hits the L1 or L2): 5001 rows of bf16 30 us for 113 MB.
 template <typename T, typename O, bool kDense>
 __device__ __forceinline__ void append_body(const Kv8AppendParams& p) {
@@ -287,8 +287,8 @@ __global__ void __launch_bounds__(128, 12) kv8_append_dense_kernel(Kv8AppendPara
 }
 
 // grid (min(n, 64), layers, 2 * Hkv): one page and head per block and step, 2 KB for 16 slots, so that a
-// fork of a few pages spreads over the device (9 pages in 16 layers, 8 kv heads: 6.5 us for 9.4 MB read and
-// written, launch included).  Copies of one call are independent: a destination that is
+// fork of a few pages spreads over the device (9 pages in 16 layers, 8 kv heads: 6.5 us with the read-back of
+// the copies, 24 MB in all).  Copies of one call are independent: a destination that is
 // also a source, or twice a destination, is reported and skipped.  The slots behind the copied ones
 // are zeroed; a copy of no token leaves an empty page (scale 0), which is how a page is freed.
 __global__ void __launch_bounds__(128)
@@ -320,7 +320,8 @@ __global__ void __launch_bounds__(128)
 
 // grid (layers, 2 * Hkv), 256 threads; shared memory: n codes rows, scales, slots, page tables.
 // Every source is read before any slot is written; then one warp per destination page, which may have to
-// round its other slots again.  Bound by latency, three dependent trips to memory (4 moves in 32 layers 7.3 us).
+// round its other slots again.  Bound by latency, three dependent trips to memory (4 moves in 32 layers 7.3 us with the pages
+// read back).
 __global__ void __launch_bounds__(256)
     kv8_move_slots_kernel(uint8_t* __restrict__ data, float* __restrict__ scale, const int* __restrict__ src,
                           const int* __restrict__ dst, int n, int num_pages, int Hkv, int page_shift, int* err) {
