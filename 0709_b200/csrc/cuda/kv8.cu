@@ -122,7 +122,9 @@ __device__ __forceinline__ void load_kv8(const Kv8AppendParams& p, int r, int po
 }
 
 // One kv head of `page`, which row m writes, if m is the first row of the batch to write it: all of the
-// page's rows.  So each page and head has one writer and no order of blocks matters.
+// page's rows.  So each page and head has one writer and no order of blocks matters.  The price is that
+// every such block looks through all slots: about a fifth of the time at 16384 rows (138 us with the pages
+// read back, 3.5 times that of 5001 rows), growing with the square of the rows.
 template <typename T, bool kDense>
 __device__ __forceinline__ void append_page(const Kv8AppendParams& p, int m, int page, int h) {
   __shared__ int owner[kMaxPage];  // row that writes slot o, -1: none
