@@ -161,8 +161,11 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
   uint64_t* s_full = empty16 + kStages16;  // [slot][buffer]
   // [slot][buffer], 128 arrivals: a warp may write P(k + 1) while another still works on P(k)
   uint64_t* p_full = s_full + 4;
-  uint64_t* pv_done = p_full + 4;          // [2]
-  uint64_t* q_full = pv_done + 2;          // every staging thread
+  uint64_t* pv_done = p_full + 4;          // [2], a phase per P V product but the last
+  // [2], one phase: the slot's last product.  A warp may leave the loop while the product before the last is
+  // still to run (its last S proves only the third from last), and a parity of pv_done could not tell the two.
+  uint64_t* fin = pv_done + 2;
+  uint64_t* q_full = fin + 2;              // every staging thread
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_full + 1);
   int8_t* q_exp = reinterpret_cast<int8_t*>(full8) + 256;  // [256] exponent that scaled each row of Q
 
@@ -190,6 +193,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
       mbar_init(&p_full[2 * s], 128);
       mbar_init(&p_full[2 * s + 1], 128);
       mbar_init(&pv_done[s], 1);
+      mbar_init(&fin[s], 1);
     }
     mbar_init(q_full, R::kProducer * 32);
     fence_barrier_init();
@@ -409,7 +413,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               umma_f16_ts(tO, tS0 + (j & 1) * 64 + kk * 8, lo + kk * (2048 >> 4), kDescHi, idesc_o, j > 0 || kk > 0);
-            umma_commit(&pv_done[slot]);
+            umma_commit(k < n ? &pv_done[slot] : &fin[slot]);
             umma_commit(&empty16[d]);
           }
           __syncwarp();
@@ -492,7 +496,9 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
           ref = top;
           sum *= a;
         }
-        if (k > 0) {  // O has to hold P V of every chunk before
+        // O has to hold P V of every chunk before; S(k) was started after product k - 2, so the phase of
+        // product k - 1 is the one that its parity names.
+        if (k > 0) {
           ok = wait8(&pv_done[slot], (k - 1) & 1, p.err) && ok;
           __syncwarp();
           tc_fence_after();
@@ -544,9 +550,8 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
       mbar_arrive(&p_full[slot * 2 + (k & 1)]);
     }
     // ---- epilogue
-    if (n > 0) ok = wait8(&pv_done[slot], (n - 1) & 1, p.err) && ok;
+    if (n > 0) ok = wait8(&fin[slot], 0, p.err) && ok;
     __syncwarp();
-    tc_fence_after();
     const int64_t pairs = static_cast<int64_t>(p.M) * p.Hq;
     const int64_t record = (ksplit ? 2 * blockIdx.y + slot : blockIdx.y) * pairs;
     const bool direct = p.direct != 0;
@@ -554,6 +559,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
     // O by way of shared memory (the chunks' space, once both slots are done with it): a thread lays its
     // row down and copies it out as one bulk transfer.  Rows are padded by 16 bytes against bank conflicts.
     asm volatile("bar.sync 1, 256;" ::: "memory");
+    tc_fence_after();  // the loads of O stay behind the wait above, and the rows behind both slots' products
     constexpr int kRowOut = kHd * 4 + 16;
     uint8_t* row_s = ring8 + tid * kRowOut;
     const bool any = n > 0 && sum != 0.f;
