@@ -70,7 +70,7 @@ __device__ __forceinline__ void fold_tail8(const Attn8Params& p, const Attn8Shap
         decode4(kw[u], k);
         decode4(vw[u], v);
         const float dot = warp_sum(q[0] * k[0] + q[1] * k[1] + q[2] * k[2] + q[3] * k[3]);
-        const float s2 = fmaf(dot, c.x * p.scale_log2, c.y);
+        const float s2 = fmaf(dot, attn8_factor(p.scale_log2, c.x), c.y);
         const float nm = fmaxf(ref, s2);
         const float a = ref > -INFINITY ? ex2(ref - nm) : 0.f, w = ex2(s2 - nm);
 #pragma unroll
@@ -338,9 +338,11 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int nt = 0; nt < 2; ++nt) {
+          const float f = attn8_factor(fac[mt][e], kf[nt]);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) s[mt][nt][e * 2 + k] = fmaf(s[mt][nt][e * 2 + k], fac[mt][e] * kf[nt], lv[nt]);
+          for (int k = 0; k < 2; ++k) s[mt][nt][e * 2 + k] = fmaf(s[mt][nt][e * 2 + k], f, lv[nt]);
+        }
         if (masked) {
           const int grow = tile0 + mt * 16 + e * 8 + g;
           uint32_t vis = 0;

@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
           float mx = max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), fmaxf(v[6], v[7]));
           if constexpr (kGroup == 16)
             mx = max3(mx, max3(max3(v[8], v[9], v[10]), v[11], v[12]), max3(v[13], v[14], v[15]));
-          top = fmaxf(top, fmaf(mx, fac * w.x, w.y));
+          top = fmaxf(top, fmaf(mx, attn8_factor(fac, w.x), w.y));
         }
       };
       if constexpr (ksplit) {
@@ -519,7 +519,8 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
 #pragma unroll
         for (int gk = 0; gk < 4; gk += kGroup / 8) {
           const float4 w = sc[half * 4 + gk];
-          const uint64_t f = pair2(fac * w.x, fac * w.x), b = pair2(w.y + neg, w.y + neg);
+          const float fk = attn8_factor(fac, w.x);
+          const uint64_t f = pair2(fk, fk), b = pair2(w.y + neg, w.y + neg);
           uint64_t acc = 0;
 #pragma unroll
           for (int j = 0; j < kGroup; j += 2) {
