@@ -7,7 +7,8 @@
 //
 // The weights carry V's scale: with u = score * log2(e) + log2(v_scale) a key adds 2^(u - ref) * code_v
 // to O and 2^(u - ref) / v_scale to the sum, ref following the largest u, so pages of very different
-// size meet in one accumulator without overflow.
+// size meet in one accumulator without overflow.  The split passes round the weights of O to fp16 (11 bits
+// for codes of 4) and sum them in fp32.
 
 #include <cuda_fp8.h>
 
@@ -359,16 +360,17 @@ __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
         }
         top[e] = fmaxf(fmaxf(s[mt][0][e * 2], s[mt][0][e * 2 + 1]), fmaxf(s[mt][1][e * 2], s[mt][1][e * 2 + 1]));
       }
-      // ref follows the row's largest u only when that grew by more than 8 (a factor of 256): P stays
-      // far inside fp16, and O is rarely rescaled.
-      if (__any_sync(0xffffffffu, top[0] > ref[mt][0] + 8.f || top[1] > ref[mt][1] + 8.f)) {
+      // ref follows the row's largest u only when that grew by more than 8 (a factor of 256): O is rarely
+      // rescaled.
+      if (__any_sync(0xffffffffu, ref_moves(top[0], ref[mt][0]) || ref_moves(top[1], ref[mt][1]))) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float mx = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          if (mx > ref[mt][e] + 8.f) {
-            const float a = ref[mt][e] > -INFINITY ? ex2(ref[mt][e] - mx) : 0.f;
-            ref[mt][e] = mx;
+          if (ref_moves(mx, ref[mt][e])) {
+            const float to = mx - kTopWeight;
+            const float a = ref[mt][e] > -INFINITY ? ex2(ref[mt][e] - to) : 0.f;
+            ref[mt][e] = to;
             sum[mt][e] *= a;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {

@@ -11,6 +11,14 @@ namespace {
 constexpr int kHd = 128;
 }  // namespace
 
+// Weights are rounded to fp16, 2^(u - ref).  The reference is set 7 below a row's largest u and moves when a weight
+// would pass 2^15, so that the largest weight is at least 2^7 and what fp16 loses at its lower end (2^-25) is below
+// 2^-32 of it: a million such keys hold less than a quarter of a thousandth of the row.  (Set to the largest u itself,
+// keys below 2^-25 of it vanished from O and stayed in the sum.)
+constexpr float kTopWeight = 7.f;
+constexpr float kMaxWeight = 15.f;
+__device__ __forceinline__ bool ref_moves(float top, float ref) { return top - ref > kMaxWeight; }
+
 struct Attn8Shape {
   int shared_len, n_shared, mask_base, shared_end;
 };

@@ -48,7 +48,6 @@ struct Roles {
 };
 constexpr int kSmem = 1024 + 4 * kBytes8 + kStages16 * kBytes16 + kBytesQ + (4 + kStages16) * 128 + 256 + 256;
 constexpr uint32_t kColO = 256;
-constexpr float kGrow = 14.f;  // log2: P stays <= 2^14 between rescales (fp16 ends at 2^16)
 }  // namespace
 
 // D (+)= A(tmem) * B(smem); B's descriptor as two words, so that the tiles of one operand differ by
@@ -488,12 +487,13 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
 #pragma unroll
         for (int half = 0; half < 2; ++half) half_top(half, s[half % kKept]);
       }
-      const bool grow_ref = top > ref + kGrow;
-      if (__any_sync(0xffffffffu, grow_ref)) {
+      const bool moves = ref_moves(top, ref);
+      if (__any_sync(0xffffffffu, moves)) {
         float a = 1.f;
-        if (grow_ref) {
-          a = ref > -INFINITY ? ex2(ref - top) : 0.f;
-          ref = top;
+        if (moves) {
+          const float to = top - kTopWeight;
+          a = ref > -INFINITY ? ex2(ref - to) : 0.f;
+          ref = to;
           sum *= a;
         }
         // O has to hold P V of every chunk before; S(k) was started after product k - 2, so the phase of
