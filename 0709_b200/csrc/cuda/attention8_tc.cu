@@ -22,6 +22,8 @@
 // 1750 (two share a scheduler), the converters for 880.  The short calls are bound by their start: a CTA's
 // first scores come about 6000 cycles after its launch, O leaves 2000 after its last chunk.
 
+#include <type_traits>
+
 #include "attention8.cuh"
 
 namespace atlas {
@@ -443,7 +445,11 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
     const int n = ksplit ? (chunks + 1 - slot) / 2 : chunks;
     float ref = -INFINITY, sum = 0.f;
     bool ok = true;
-    for (int k = 0; k < n && __all_sync(0xffffffffu, ok); ++k) {
+    // One chunk.  Once a row's reference is beyond 2^20, u - ref has to be taken from the rounded u, as the maximum
+    // was (in one step the two can differ by more than fp16 holds): the plain form returns false and leaves the chunk
+    // to the far one, which is kept small (4 us of the 2048-row chunk; as a branch within one form 10 us).
+    auto fold_chunk = [&](auto far_form, int k) {
+      constexpr bool kFar = decltype(far_form)::value;
       const int c = ksplit ? 2 * k + slot : k;
       const int d = c % kStages16;
       ok = wait8(&s_full[slot * 2 + (k & 1)], (k >> 1) & 1, p.err);
@@ -458,7 +464,8 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
       const float4* sc = sc16 + d * 8;
       // S 32 keys at a time.  With eight converter warps a row of S does not fit the registers and is read
       // twice, for the maximum and for the weights; with four it stays.
-      constexpr int kKept = ksplit ? 1 : 2;
+      constexpr bool kTwice = ksplit || kFar;
+      constexpr int kKept = kTwice ? 1 : 2;
       float s[kKept][32];
       float top = -INFINITY;
       auto load_half = [&](int half, float* v) {
@@ -475,7 +482,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
           top = fmaxf(top, fmaf(mx, attn8_factor(fac, w.x), w.y));
         }
       };
-      if constexpr (ksplit) {
+      if constexpr (kTwice) {
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           load_half(half, s[0]);
@@ -488,6 +495,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
         for (int half = 0; half < 2; ++half) half_top(half, s[half % kKept]);
       }
       const bool moves = ref_moves(top, ref);
+      bool far = false;
       if (__any_sync(0xffffffffu, moves)) {
         float a = 1.f;
         if (moves) {
@@ -496,6 +504,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
           ref = to;
           sum *= a;
         }
+        if constexpr (!kFar) far = __any_sync(0xffffffffu, ref > -INFINITY && fabsf(ref) > 0x1p20f);
         // O has to hold P V of every chunk before; S(k) was started after product k - 2, so the phase of
         // product k - 1 is the one that its parity names.
         if (k > 0) {
@@ -512,6 +521,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
           }
         }
       }
+      if (far) return false;
       const float neg = ref > -INFINITY ? -ref : 0.f;
       __syncwarp();
       auto weigh_half = [&](int half, const float* v) {
@@ -519,15 +529,15 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
 #pragma unroll
         for (int gk = 0; gk < 4; gk += kGroup / 8) {
           const float4 w = sc[half * 4 + gk];
-          const float fk = attn8_factor(fac, w.x);
-          const uint64_t f = pair2(fk, fk), b = pair2(w.y + neg, w.y + neg);
+          const float f1 = attn8_factor(fac, w.x), b1 = kFar ? w.y : w.y + neg;
+          const uint64_t f = pair2(f1, f1), b = pair2(b1, b1);
           uint64_t acc = 0;
 #pragma unroll
           for (int j = 0; j < kGroup; j += 2) {
             float p0, p1;
             unpair2(fma2(pair2(v[gk * 8 + j], v[gk * 8 + j + 1]), f, b), p0, p1);
-            p0 = ex2(p0);
-            p1 = ex2(p1);
+            p0 = ex2(kFar ? p0 + neg : p0);
+            p1 = ex2(kFar ? p1 + neg : p1);
             acc = add2(acc, pair2(p0, p1));
             pk[gk * 4 + j / 2] = __uint_as_float(pack_half2(p0, p1));
           }
@@ -537,7 +547,7 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
         }
         tmem_st16(tS + half * 16, pk);  // over keys of the first half, which are read
       };
-      if constexpr (ksplit) {
+      if constexpr (kTwice) {
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           load_half(half, s[0]);
@@ -549,7 +559,11 @@ __global__ void __launch_bounds__(Roles<kSplitKeys>::kThreads, 1)
       }
       tc_fence_before();
       mbar_arrive(&p_full[slot * 2 + (k & 1)]);
-    }
+      return true;
+    };
+    int k = 0;
+    while (k < n && __all_sync(0xffffffffu, ok) && fold_chunk(std::false_type{}, k)) ++k;
+    for (; k < n && __all_sync(0xffffffffu, ok); ++k) fold_chunk(std::true_type{}, k);
     // ---- epilogue
     if (n > 0) ok = wait8(&fin[slot], 0, p.err) && ok;
     __syncwarp();

@@ -183,3 +183,46 @@ def test_scores_that_rise_along_the_keys(rows, hq, hkv, keys):
     tol += keys * 2.0 ** -30 * p.amax(-1, keepdim=True) * v.abs().max()
     diff = (out.double().reshape(want.shape) - want).abs()
     assert bool((diff <= tol).all()), float((diff / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("step", [16, 32])
+@pytest.mark.parametrize("rows,hq,hkv,keys", LONG)
+def test_scores_beyond_the_steps_of_a_binade(rows, hq, hkv, keys, step):
+    """Scores of 1.5 * 2^25 binades, where fp32 goes by fours, and every seventh chunk from the third on has keys that
+    lie ``step`` higher: sums of two products 2^22 apart at most, exact in fp32, so that the weights are."""
+    ops = impl("cuda")
+    cache, n, k, v, pages, g = long_cache(hkv, keys)
+    k.zero_()
+    k[..., 0] = 1.5 * 2.0 ** 17
+    k[8::28, :, ::5, 1] = float(step)
+    v = v.clamp(-1.75, 1.75)
+    v[:, :, 0, 0] = 1.75  # every page's v scale is 2^-8: u stays a multiple of four
+    store(cache, pages, k, v)
+    q = torch.zeros(rows, hq, 128, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 2.0 ** 8
+    q[..., 1] = 1
+    lens = torch.full((rows,), keys, dtype=torch.int32, device="cuda")
+    out = ops.attention8(q, cache.layer(0), mod("ops.attn_desc").single_sequence_desc(pages, lens, keys), math.log(2))
+    settle(ops)
+    want, p, mag, v = dense(q, cache.layer(0), pages, torch.arange(keys, device="cuda") < lens[:, None], math.log(2))
+    tol = mag * (2.0 ** -11 + 2.0 ** -16) + want.abs() * 2.0 ** -8 + 2.0 ** -24
+    tol += keys * 2.0 ** -32 * p.amax(-1, keepdim=True) * v.abs().max()
+    diff = (out.double().reshape(want.shape) - want).abs()
+    assert bool((diff <= tol).all()), float((diff / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** 11, 2.0 ** 12, 2.0 ** 13, 2.0 ** 14])
+@pytest.mark.parametrize("rows,hq,hkv,keys", LONG)
+def test_scores_that_fp32_cannot_resolve(rows, hq, hkv, keys, size):
+    """Scores around 2^23 to 2^29 binades, off by whole binades in any 32-bit form: the answer stays an average of the
+    values."""
+    ops = impl("cuda")
+    cache, n, k, v, pages, g = long_cache(hkv, keys)
+    store(cache, pages, k * size, v)
+    q = (torch.randn(rows, hq, 128, device="cuda", generator=g) * size).bfloat16()
+    lens = torch.full((rows,), keys, dtype=torch.int32, device="cuda")
+    out = ops.attention8(q, cache.layer(0), mod("ops.attn_desc").single_sequence_desc(pages, lens, keys))
+    settle(ops)
+    assert bool((out.float().abs() <= cache.layer(0).values()[:, 1].abs().max() * (1 + 2.0 ** -7)).all())
