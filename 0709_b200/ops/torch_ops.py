@@ -108,6 +108,8 @@ def _row_positions(desc: AttnDesc, r: int, page_size: int) -> tuple[torch.Tensor
     pages[shared] = desc.prefix_pages.long()[j[shared]]
     if (~shared).any():
         pages[~shared] = desc.tail_pages[r].long()[j[~shared] - desc.n_shared_pages]
+    if bool((pages < 0).any()):
+        raise IndexError(f"row {r} reads a negative page")
     return pos, pages * page_size + pos % page_size
 
 
@@ -227,6 +229,8 @@ def kv8_read_pages(cache: kv8.Kv8Cache | kv8.Kv8Layer, pages: torch.Tensor, dtyp
     largest finite value of ``dtype``)."""
     idx = pages.long()
     data, scale = cache.data.view(torch.uint8), cache.scale
+    if bool((idx < 0).any()):
+        raise IndexError("negative page")
     if isinstance(cache, kv8.Kv8Cache):
         data, scale = data[:, idx], scale[:, idx]
     else:
