@@ -96,10 +96,12 @@ def _row_positions(desc: AttnDesc, r: int, page_size: int) -> tuple[torch.Tensor
     full = int(desc.row_full[r])
     vis = pos < full
     if n > full:
-        rel = (pos - desc.mask_base).clamp(min=0)
+        rel = pos - desc.mask_base
         words = desc.row_mask[r]
-        word = words[(rel // 64).clamp(max=words.numel() - 1)]
-        bit = torch.bitwise_and(torch.bitwise_right_shift(word, rel % 64), 1).bool()
+        inside = (rel >= 0) & (rel < 64 * words.numel())  # no bit, no key
+        rel = rel[inside]
+        bit = torch.zeros_like(vis)
+        bit[inside] = torch.bitwise_and(torch.bitwise_right_shift(words[rel // 64], rel % 64), 1).bool()
         vis = vis | ((pos >= full) & bit)
     pos = pos[vis]
     j = pos // page_size
