@@ -306,6 +306,8 @@ class CudaOps:
     # no workspace is shared between streams, calls or captured graphs.
     @staticmethod
     def _int32(t: torch.Tensor) -> torch.Tensor:
+        if t.dtype == torch.int64:  # what does not fit stays out of every range: the kernels report it
+            t = t.clamp(-1, 2 ** 31 - 1)
         return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
     def rope_qkv_append8(self, qkv, table, positions, slots, kv_layer, num_heads, num_kv_heads, out_dtype=None):

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from conftest import mod
-from test_kv8 import Oracle, check_attention, impl, make_cache, settle
+from test_kv8 import Oracle, assert_pages, check_attention, impl, make_cache, rope, settle
 from test_kv8_limits import IMPLS, ints, reported
 
 
@@ -48,3 +48,59 @@ def test_keys_outside_the_mask(device, rows, hq, words):
     out = ops.attention8(q.to(device), cache.layer(0), desc)
     settle(ops)
     check_attention(out, q, Oracle(cache).val[0], desc, 1 / math.sqrt(128))
+
+
+def longs(x, device):
+    return torch.tensor(x, dtype=torch.int64, device=device)
+
+
+FAR = [2 ** 32 + 3, -2 ** 32 + 3, 2 ** 40, -1]  # the first two are 3 in their low 32 bits
+
+
+@pytest.mark.parametrize("device", IMPLS)
+@pytest.mark.parametrize("bad", FAR)
+def test_append_indices_beyond_32_bits(device, bad):
+    cache = make_cache(device, 1, 6, 1, 16, 128, seed=0)
+    before = Oracle(cache)
+    qkv, table = torch.randn(1, 3 * 128, device=device), rope(8, 128, device)
+    for pos, slot in ((0, bad), (bad, 3)):
+        reported(device, lambda ops: ops.rope_qkv_append8(qkv, table, longs([pos], device), longs([slot], device),
+                                                          cache.layer(0), 1, 1), 2)
+        assert_pages(cache, before)
+
+
+@pytest.mark.parametrize("device", IMPLS)
+@pytest.mark.parametrize("bad", FAR)
+def test_page_indices_beyond_32_bits(device, bad):
+    cache = make_cache(device, 2, 6, 2, 16, 128, seed=0)
+    before = Oracle(cache)
+    for src, dst in ((bad, 5), (5, bad)):
+        reported(device, lambda ops: ops.kv8_move_slots(cache, longs([src], device), longs([dst], device)), 2)
+    for plan in ((bad, 1, 2), (1, bad, 2), (1, 2, bad)):
+        reported(device, lambda ops: ops.kv8_copy_pages(cache, longs([plan], device)), 2)
+    assert_pages(cache, before)
+
+
+@pytest.mark.parametrize("device", IMPLS)
+@pytest.mark.parametrize("bad", FAR)
+def test_read_pages_beyond_32_bits(device, bad):
+    cache = make_cache(device, 2, 6, 2, 16, 128, seed=0)
+    for what in (cache, cache.layer(1)):
+        reported(device, lambda ops: ops.kv8_read_pages(what, longs([2, bad], device), torch.float16), 2)
+
+
+@pytest.mark.parametrize("device", IMPLS)
+def test_indices_of_64_bits(device):
+    """The same indices in 64 bits and in 32 give the same cache."""
+    ops = impl(device)
+    caches = [make_cache(device, 1, 6, 1, 16, 128, seed=0) for _ in range(2)]
+    qkv, table = torch.randn(3, 3 * 128, device=device), rope(8, 128, device)
+    for cache, make in zip(caches, (ints, longs)):
+        ops.rope_qkv_append8(qkv, table, make([5, 6, 7], device), make([14, 15, 16], device), cache.layer(0), 1, 1)
+        ops.kv8_move_slots(cache, make([16], device), make([40], device))
+        ops.kv8_copy_pages(cache, make([[0, 4, 9]], device))
+    settle(ops)
+    assert torch.equal(caches[0].scale, caches[1].scale)
+    assert torch.equal(caches[0].data.view(torch.uint8), caches[1].data.view(torch.uint8))
+    pages = [ops.kv8_read_pages(caches[0], make([4, 1], device), torch.float16) for make in (ints, longs)]
+    assert torch.equal(*pages)
