@@ -134,6 +134,10 @@ class LlamaEngine:
     def _move(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         self.ops.kv_move_slots(self.kv, src, dst)
 
+    def read_pages(self, pages: torch.Tensor) -> torch.Tensor:
+        """K and V of ``pages``: [layers, n, 2, kv_heads, page_size, head_dim] in the engine's dtype."""
+        return self.kv[:, pages.to(self.device, torch.long)]
+
     # ------------------------------------------------------------------
     def _fold_norms(self):
         """Weights with the RMSNorm gains multiplied into their input columns.

@@ -61,6 +61,9 @@ class _Kv8Cache:
     def _move(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         self.ops.kv8_move_slots(self.kv, src, dst)
 
+    def read_pages(self, pages: torch.Tensor) -> torch.Tensor:
+        return self.ops.kv8_read_pages(self.kv, pages.to(self.device), self.dtype)
+
 
 class Kv8LlamaEngine(_Kv8Cache, LlamaEngine):
     """16-bit weights (fp32 on CPU), 8-bit cache."""

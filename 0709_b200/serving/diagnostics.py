@@ -29,6 +29,8 @@ import sys
 
 import torch
 
+from ..runtime.engine_kv8 import KV_CACHES, make_engine
+
 _INERT = (("--mem-fraction-static", float), ("--max-running-requests", int), ("--max-total-tokens", int),
           ("--nccl-port", int), ("--workspace-mb", int))
 
@@ -42,6 +44,8 @@ def _common(p) -> None:
     p.add_argument("--page-size", type=int, default=16)
     p.add_argument("--context-length", type=int, default=8192)
     p.add_argument("--dtype", default="float16", choices=["float16", "bfloat16", "float32"])
+    p.add_argument("--kv-cache", choices=KV_CACHES, default="model",
+                   help="Precision of the KV cache: the model's, or fp8 (K and V rounded to 4 significant bits).")
     p.add_argument("--device", default=None)
     p.add_argument("--gpu-id", type=int, default=None)
     p.add_argument("--seed", type=int, default=0)
@@ -97,21 +101,19 @@ def _prompt(args, vocab: int) -> list[int]:
 
 
 def _engine(w, args):
-    from ..runtime.engine import LlamaEngine
-
     ctx = int(args.context_length)
-    return LlamaEngine(w, num_pages=2 * math.ceil(ctx / args.page_size) + 64, page_size=args.page_size,
-                       max_positions=ctx)
+    return make_engine(w, kv_cache=args.kv_cache, num_pages=2 * math.ceil(ctx / args.page_size) + 64,
+                       page_size=args.page_size, max_positions=ctx)
 
 
 def prefix_kv(engine, pages: list[int], n: int) -> torch.Tensor:
     """K/V of the first ``n`` positions through the page table ``pages``: [layers, 2, n, heads, dim]."""
-    ps = engine.page_size
-    pos = torch.arange(n, device=engine.kv.device)
-    page = torch.tensor(pages, device=engine.kv.device, dtype=torch.long)[pos // ps]
-    # kv: [layers, pages, 2, kv_heads, page_size, head_dim]; the two index tensors are not adjacent,
-    # so their (position) dimension comes first: [n, layers, 2, kv_heads, head_dim].
-    return engine.kv[:, page, :, :, pos % ps, :].permute(1, 2, 0, 3, 4)
+    need = -(-n // engine.page_size)
+    if need > len(pages):
+        raise IndexError(f"{n} positions need {need} pages of {engine.page_size}; the table has {len(pages)}")
+    kv = engine.read_pages(torch.tensor(pages[:need], dtype=torch.int32))
+    layers, _, sides, heads, _, dim = kv.shape
+    return kv.permute(0, 2, 1, 4, 3, 5).reshape(layers, sides, -1, heads, dim)[:, :, :n]
 
 
 def target_commit(args) -> dict:
