@@ -168,6 +168,10 @@ def rope_qkv_append8(
     """Rotate q/k, write k and v into the 8-bit cache at ``slots``; return rotated q [M, Hq, hd]."""
     m = qkv.shape[0]
     hd = kv_layer.data.shape[-1]
+    if num_kv_heads != kv_layer.data.shape[2]:
+        raise ValueError(f"{num_kv_heads} kv heads for a cache of {kv_layer.data.shape[2]}")
+    if positions.numel() != m or slots.numel() != m:
+        raise ValueError(f"{positions.numel()} positions and {slots.numel()} slots for {m} rows")
     x = qkv.float().reshape(m, num_heads + 2 * num_kv_heads, hd)
     if m and not bool(((positions >= 0) & (positions < table.shape[0])).all()):
         raise IndexError(f"position outside the rotary table of {table.shape[0]}")
@@ -218,6 +222,8 @@ def kv8_move_slots(cache: kv8.Kv8Cache, src_slots: torch.Tensor, dst_slots: torc
     """Move slot contents (all layers, k and v); sources are read before any write.  A row needs its source
     page's scale."""
     pages, ps = cache.data.shape[1], cache.data.shape[-2]
+    if src_slots.numel() != dst_slots.numel():
+        raise ValueError(f"{src_slots.numel()} source slots for {dst_slots.numel()} destinations")
     if src_slots.numel() and not bool(((src_slots >= 0) & (src_slots < pages * ps)).all()):
         raise IndexError(f"source slot outside the cache of {pages} pages of {ps} slots")
     sp, so = _slot_to_page(src_slots, ps)

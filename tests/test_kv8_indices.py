@@ -104,3 +104,23 @@ def test_indices_of_64_bits(device):
     assert torch.equal(caches[0].data.view(torch.uint8), caches[1].data.view(torch.uint8))
     pages = [ops.kv8_read_pages(caches[0], make([4, 1], device), torch.float16) for make in (ints, longs)]
     assert torch.equal(*pages)
+
+
+@pytest.mark.parametrize("device", IMPLS)
+def test_arguments_that_do_not_fit_together(device):
+    """Kv heads that are not the cache's, and lists of different lengths."""
+    ops = impl(device)
+    cache = make_cache(device, 1, 6, 2, 16, 128, seed=0)
+    before = Oracle(cache)
+    table, layer = rope(8, 128, device), cache.layer(0)
+    one, two = ints([1], device), ints([1, 2], device)
+    qkv = torch.randn(2, 6 * 128, device=device).half()
+    for call in (lambda: ops.rope_qkv_append8(qkv, table, two, two, layer, 4, 1),
+                 lambda: ops.rope_qkv_append8(qkv, table, one, two, layer, 2, 2),
+                 lambda: ops.rope_qkv_append8(qkv, table, two, one, layer, 2, 2),
+                 lambda: ops.kv8_move_slots(cache, two, one),
+                 lambda: ops.kv8_move_slots(cache, one, two)):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
+    settle(ops)
+    assert_pages(cache, before)
