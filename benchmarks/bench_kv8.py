@@ -2,6 +2,7 @@
 
     python benchmarks/bench_kv8.py                       # attention and append, 8B head geometry
     python benchmarks/bench_kv8.py --model llama-8b      # one-row and tree forwards of a model as well
+    python benchmarks/bench_kv8.py --max-positions 32768 # launches sized for a longer context, as a server's graphs are
 
 Attention: one captured graph of many calls over several layers (more cache than L2 holds from 16K keys
 on), CUDA events around its replay.  Forwards: the engines' own graphs, random-init weights, a cache of
@@ -51,7 +52,8 @@ def captured(fn, calls: int):
     return g
 
 
-def attention(rows: int, length: int, hq: int, hkv: int, page: int, dtype: torch.dtype, layers: int) -> dict:
+def attention(rows: int, length: int, hq: int, hkv: int, page: int, dtype: torch.dtype, layers: int,
+              max_positions: int) -> dict:
     cuda_ops, kv8, attn_desc = pkg("ops.cuda_ops"), pkg("ops.kv8"), pkg("ops.attn_desc")
     dev = torch.device("cuda")
     n = -(-(length + rows) // page)
@@ -71,7 +73,10 @@ def attention(rows: int, length: int, hq: int, hkv: int, page: int, dtype: torch
     desc = attn_desc.single_sequence_desc(pages, lens, length, mask_base=length, masks=masks,
                                           full=torch.full_like(lens, length))
     q = torch.randn(rows, hq, 128, device=dev).to(dtype)
-    ops.reserve_attention_workspace(rows, hq, hkv, length, page)
+    ops.reserve_attention_workspace(rows, hq, hkv, max(length, max_positions), page)
+    if max_positions > length:
+        desc._max_keys = max_positions
+        desc._splits = ops.attention_splits(rows, hq, hkv, max_positions, page)
 
     def run16():
         for i in range(layers):
@@ -88,13 +93,14 @@ def attention(rows: int, length: int, hq: int, hkv: int, page: int, dtype: torch
     return res
 
 
-def forwards(model: str, length: int, page: int) -> list[dict]:
+def forwards(model: str, length: int, page: int, max_positions: int) -> list[dict]:
     loader, e8 = pkg("models.loader"), pkg("runtime.engine_kv8")
     w = loader.resolve_model(model, dtype="float16", device="cuda", seed=0)
     pages = -(-(length + 64) // page) + 4
     out = []
     for kv_cache in ("model", "fp8"):
-        eng = e8.make_engine(w, kv_cache=kv_cache, num_pages=pages, page_size=page, max_positions=length + 128)
+        eng = e8.make_engine(w, kv_cache=kv_cache, num_pages=pages, page_size=page,
+                             max_positions=max(length + 128, max_positions))
         table = torch.arange(pages, dtype=torch.int32, device="cuda")
         tokens = torch.randint(0, w.config.vocab_size, (length,), device="cuda").int()
         a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
@@ -135,13 +141,16 @@ def main(argv=None) -> int:
     p.add_argument("--rows", type=int, nargs="+", default=[1, 4, 12, 48])
     p.add_argument("--page-size", type=int, default=16)
     p.add_argument("--layers", type=int, default=4)
+    p.add_argument("--max-positions", type=int, default=0,
+                   help="longest context that the launches are sized for (default: each length's own)")
     a = p.parse_args(argv)
     for length in a.lengths:
         for rows in a.rows:
-            print(json.dumps(attention(rows, length, 32, 8, a.page_size, torch.float16, a.layers)), flush=True)
+            print(json.dumps(attention(rows, length, 32, 8, a.page_size, torch.float16, a.layers,
+                                       a.max_positions)), flush=True)
     if a.model:
         for length in a.lengths:
-            for r in forwards(a.model, length, a.page_size):
+            for r in forwards(a.model, length, a.page_size, a.max_positions):
                 print(json.dumps(r), flush=True)
     return 0
 
