@@ -124,3 +124,22 @@ def test_arguments_that_do_not_fit_together(device):
             call()
     settle(ops)
     assert_pages(cache, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 70])
+def test_a_refused_row_that_repeats_a_slot(rows):
+    """The later row of a slot counts, also where it cannot be stored: the slot keeps what it held, the rows beside it
+    are stored."""
+    cache = make_cache("cuda", 1, 8, 1, 16, 128, seed=rows)
+    oracle = Oracle(cache)
+    qkv = torch.ones(rows, 3 * 128, device="cuda")
+    qkv[rows - 1, 300] = math.nan
+    slots = list(range(17, 17 + rows - 1)) + [17]
+    reported("cuda", lambda ops: ops.rope_qkv_append8(qkv, rope(4, 128, "cuda"), ints([0] * rows, "cuda"),
+                                                      ints(slots, "cuda"), cache.layer(0), 1, 1), 5)
+    row = (torch.ones(128, dtype=torch.float64), 2.0 ** -8)
+    for side in (0, 1):
+        for page in range(1, 8):
+            oracle.write(0, side, 0, page, {s % 16: row for s in slots[1:-1] if s // 16 == page})
+    assert_pages(cache, oracle)
