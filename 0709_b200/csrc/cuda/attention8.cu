@@ -124,6 +124,8 @@ struct SplitCfg {
 // 4.9 TB/s, 0.75 of the measured copy rate; issue slots 51 % busy, ALU 44 % (conversion), tensor pipe 32 %, so
 // that what is left is the start and the merge (5 us) and loads that stop while a warp converts.  Separate
 // accumulators for the two 64-dimension halves of S, to shorten its chain of products, spilled (56 us).
+// Short calls: 36 rows a kv head on 2051 keys take 4100 cycles to the first products, 5500 for two units per
+// warp and 4200 to join the warps, then 3.6 us of merge (13.3 us in all).
 template <typename T, int MT>
 __global__ void __launch_bounds__(256, MT == 1 ? 2 : 1)
     attn8_split_kernel(const __grid_constant__ CUtensorMap map, Attn8Params p) {

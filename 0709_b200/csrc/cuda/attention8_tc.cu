@@ -15,12 +15,14 @@
 //
 // TMEM columns: S/P of slot s, buffer b at 128 s + 64 b; O of slot s at 256 + 128 s.
 //
-// Measured: 2048 rows x 32 heads behind 6001 keys (8 kv heads) 259 us, 0.57 of the measured bf16 matrix rate;
-// 192 rows a head on 16384 keys 34.8 us and 104 rows on 33001 keys 41.8 us with the merge.  What bounds it,
-// from cycle stamps of the first: a chunk takes 2120 cycles; the tensor pipe works for 1580 of them (an S
+// Measured: 2048 rows x 32 heads behind 6001 keys (8 kv heads) 267 us, 0.54 of the measured bf16 matrix rate;
+// 192 rows a head on 16384 keys 35.8 us and 104 rows on 33001 keys 42.2 us with the merge.  What bounds it,
+// from cycle stamps of the first: a chunk takes 2150 cycles; the tensor pipe works for 1580 of them (an S
 // product of 64 keys reads 6 KB of shared memory and runs at half rate: 65 cycles for 32), a softmax warp for
-// 1750 (two share a scheduler), the converters for 880.  The short calls are bound by their start: a CTA's
-// first scores come about 6000 cycles after its launch, O leaves 2000 after its last chunk.
+// 1700 (two share a scheduler), the converters for 880.  The short calls are bound by their ends (stamps in a
+// replayed graph): with 256 rows a CTA's first scores come 11000 cycles (five chunks of keys in all) to 14400
+// cycles (16K keys) after its launch, most of it Q, whose 24 rows per warp are loaded in three trips; with 128
+// rows 11400, 6200 of them Q.  O takes 4400 to 8000 cycles from the last chunk to the last byte.
 
 #include <type_traits>
 

@@ -18,7 +18,13 @@ returns to the pool needs no clearing: its next owner's first token starts it an
 
 The same operators exist in ``ops.torch_ops`` (any device, any head dimension; they raise where a
 row cannot be stored) and as kernels in ``ops.cuda_ops.CudaOps`` (head dimension 128, pages of 8 to 64
-slots; they report through the device error flag and leave that row out).
+slots; they report through the device error flag and leave that row out).  A row left out writes no slot:
+its page does not start anew for it, and where it repeated a slot the earlier row is not stored either.
+Indices may be int32 or int64.
+
+Attention holds the rows of q as fp16 after a power of two is taken out of each (elements below 2^-24 of a
+row's largest are lost) and rounds the weights of V's codes (softmax weight times the page's v scale) to
+fp16: 11 bits down to 2^-21 of the row's largest, fewer below, none under 2^-32 of it.  Statistics, sums and accumulators are fp32, the output is rounded once.
 """
 
 from __future__ import annotations
