@@ -348,7 +348,7 @@ class CudaOps:
 
     def kv8_copy_pages(self, cache, copies: torch.Tensor) -> None:
         """Fork: rows (src page, dst page, ntok) of ``copies``; every layer, scales included."""
-        self.ext.kv8_copy_pages(cache.data, cache.scale, self._int32(copies.to(self.device)), None, self.err)
+        self.ext.kv8_copy_pages(cache.data, cache.scale, self._int32(copies).to(self.device), None, self.err)
         counters.launches(1)
 
     def kv8_copy_pages_counted(self, cache, plan: torch.Tensor, count: torch.Tensor) -> None:
@@ -358,8 +358,8 @@ class CudaOps:
 
     def kv8_move_slots(self, cache, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Compaction: slot contents move in every layer, sources read before any write; at most 1024 moves."""
-        self.ext.kv8_move_slots(cache.data, cache.scale, self._int32(src.to(self.device)),
-                                self._int32(dst.to(self.device)), self.err)
+        self.ext.kv8_move_slots(cache.data, cache.scale, self._int32(src).to(self.device),
+                                self._int32(dst).to(self.device), self.err)
         counters.launches(1)
 
     def kv8_read_pages(self, cache, pages: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
