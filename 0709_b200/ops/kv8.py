@@ -24,7 +24,8 @@ Indices may be int32 or int64.
 
 Attention holds the rows of q as fp16 after a power of two is taken out of each (elements below 2^-24 of a
 row's largest are lost) and rounds the weights of V's codes (softmax weight times the page's v scale) to
-fp16: 11 bits down to 2^-21 of the row's largest, fewer below, none under 2^-32 of it.  Statistics, sums and accumulators are fp32, the output is rounded once.
+fp16: 11 bits down to 2^-21 of the row's largest, fewer below, none under 2^-32 of it.  Statistics, sums
+and accumulators are fp32, the output is rounded once.
 """
 
 from __future__ import annotations
@@ -47,10 +48,6 @@ class Kv8Cache:
 
     def __getitem__(self, index: int) -> Kv8Layer:
         return self.layer(index)
-
-    @property
-    def nbytes(self) -> int:
-        return self.data.numel() + 4 * self.scale.numel()
 
 
 @dataclass
